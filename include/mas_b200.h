@@ -55,6 +55,7 @@ extern "C" {
 #define MAS_STATUS_ROPE_POS_OUT_OF_RANGE 2 /* a position outside [0, max_positions): token left as is */
 #define MAS_STATUS_COPY_TIMEOUT 4          /* a bulk-copy wait ran past its time limit; outputs undefined */
 #define MAS_STATUS_KV_SLOT_OUT_OF_RANGE 8  /* a paged-KV slot index out of range: that token not appended */
+#define MAS_STATUS_KV_ALLOC_REFUSED 16     /* a page allocation or release that does not fit: nothing changed */
 
 /* Library version, (major << 16) | minor. */
 MAS_API int mas_version(void);
@@ -274,6 +275,113 @@ MAS_API int mas_rope_append_paged_kv_cache(const void* positions, int positions_
                                            int64_t k_stride_head, int64_t v_stride_token, int64_t v_stride_head,
                                            int is_neox, float q_scale_beta, int64_t q_scale_original_max,
                                            int dtype, int32_t* status, int enable_pdl, void* stream);
+
+/*
+ * Page allocation for one step of a paged KV cache, from request lengths that stay on the device.
+ * For request b of [0, batch_size): need[b] = ceil((seq_lens[b] + append_lens[b]) / page_size) -
+ * ceil(seq_lens[b] / page_size) pages; the j-th page needed, requests ascending, is
+ * free_pages[num_free[0] - 1 - j], and goes to the request's next unused entry of block_tables (row stride
+ * table_stride). seq_lens[b] += append_lens[b]; num_free[0] -= the pages taken. Outputs: cum_lens
+ * [batch_size + 1] the exclusive sum of append_lens; batch_indices / positions [max_tokens] each new token's
+ * request and position, -1 and 0 behind the last token; last_page_len [batch_size] the tokens on each request's
+ * last page (0 without tokens). All or nothing: a negative length, a table row too short, more new tokens than
+ * max_tokens, too few free pages or a num_free outside [0, free_capacity] changes neither seq_lens, block_tables
+ * nor num_free, writes cum_lens 0 and batch_indices -1, and sets MAS_STATUS_KV_ALLOC_REFUSED in *status
+ * (the library status word when status is NULL). batch_size <= 8192.
+ * Takes the place of the host-side block manager's part in ModelRunner.prepare
+ * (miniagentserve/engine/model_runner.py:31-66); the maps are those of devstral2.py:283-290.
+ */
+MAS_API int mas_allocate_paged_kv(const int32_t* append_lens, int32_t* seq_lens, int32_t* block_tables,
+                                  const int32_t* free_pages, int32_t* num_free, int32_t* cum_lens,
+                                  int32_t* batch_indices, int32_t* positions, int32_t* last_page_len,
+                                  int64_t batch_size, int64_t max_blocks, int64_t table_stride,
+                                  int64_t page_size, int64_t max_tokens, int64_t free_capacity, int32_t* status,
+                                  int enable_pdl, void* stream);
+
+/*
+ * The inverse of mas_allocate_paged_kv: cuts each request to keep_lens[b] <= seq_lens[b] tokens (0: a finished
+ * request) and gives the pages past them back. With R pages given back in all, the j-th of them (requests, then
+ * pages ascending) goes to free_pages[num_free[0] + R - 1 - j], so that releasing what was just allocated
+ * restores the list. seq_lens[b] = keep_lens[b]; num_free[0] += R; block_tables stays as it is. A keep_lens
+ * outside [0, seq_lens[b]], or a list without room, changes nothing and sets MAS_STATUS_KV_ALLOC_REFUSED.
+ */
+MAS_API int mas_release_paged_kv(const int32_t* keep_lens, int32_t* seq_lens, const int32_t* block_tables,
+                                 int32_t* free_pages, int32_t* num_free, int64_t batch_size, int64_t max_blocks,
+                                 int64_t table_stride, int64_t page_size, int64_t free_capacity, int32_t* status,
+                                 int enable_pdl, void* stream);
+
+/* One layer's paged KV cache in 4 bits. A row (one token's k or v of one kv head) is head_size codes c of 4
+ * bits, two a byte with element 2i in the low half, and a bf16 pair (scale s, minimum m); its values are
+ * c * s + m. k_codes and v_codes share sizes and strides (bytes, multiples of 16; both 16-byte aligned): entry e
+ * of page p, head h at p * stride_page + e * stride_entry + h * stride_head (NHD and HND caches alike). pairs
+ * is bf16 [num_pages][num_kv_heads][page_size][4], (k s, k m, v s, v m), pages pair_stride_page elements
+ * apart (a multiple of 4; 8-byte aligned), head-major under either layout. */
+typedef struct MasInt4KVCache {
+  void* k_codes;
+  void* v_codes;
+  void* pairs;
+  int64_t num_pages;
+  int64_t page_size;
+  int64_t stride_page;
+  int64_t stride_entry;
+  int64_t stride_head;
+  int64_t pair_stride_page;
+} MasInt4KVCache;
+
+/*
+ * mas_append_paged_kv_cache for a 4-bit cache. Each row x is stored with m = the largest bf16 <= min(x),
+ * s = the smallest bf16 >= max(2^-126, (max(x) - m) / 15), c = floor(f32(x - m) / s + 1/2). A row that holds a
+ * NaN or an infinity is stored with s = m = NaN. A token whose batch index is -1 is a padding row and is
+ * skipped; one whose indices are out of range is skipped and sets MAS_STATUS_KV_SLOT_OUT_OF_RANGE. Two tokens
+ * of one call must not name the same slot. head_size is 64 or 128; any k/v alignment and strides (16-byte
+ * aligned rows take vector loads).
+ */
+MAS_API int mas_append_paged_kv_cache_int4(const void* key, const void* value, const int32_t* batch_indices,
+                                           const void* positions, int positions_dtype, const MasInt4KVCache* cache,
+                                           const int32_t* kv_indices, int64_t num_indices,
+                                           const int32_t* kv_indptr, int64_t batch_size, int64_t num_tokens,
+                                           int64_t num_kv_heads, int64_t head_size, int64_t k_stride_token,
+                                           int64_t k_stride_head, int64_t v_stride_token, int64_t v_stride_head,
+                                           int dtype, int32_t* status, int enable_pdl, void* stream);
+
+/*
+ * Reads tokens back from a 4-bit cache: key[t, h, :] and value[t, h, :] receive c * s + m, computed in fp32 and
+ * rounded once to dtype (BF16 or FP16; a value past its largest finite one reads as that one). Indices as
+ * in the append; a padding row or an out-of-range one (MAS_STATUS_KV_SLOT_OUT_OF_RANGE) reads as zeros.
+ */
+MAS_API int mas_read_paged_kv_cache_int4(void* key, void* value, const int32_t* batch_indices,
+                                         const void* positions, int positions_dtype, const MasInt4KVCache* cache,
+                                         const int32_t* kv_indices, int64_t num_indices, const int32_t* kv_indptr,
+                                         int64_t batch_size, int64_t num_tokens, int64_t num_kv_heads,
+                                         int64_t head_size, int64_t k_stride_token, int64_t k_stride_head,
+                                         int64_t v_stride_token, int64_t v_stride_head, int dtype, int32_t* status,
+                                         int enable_pdl, void* stream);
+
+/* Bytes of workspace mas_paged_attention_int4 needs on the current device for head_size 64 or 128 (16-byte
+ * aligned; its contents matter to no later call). Two calls that may run at once need one each. */
+MAS_API int mas_paged_attention_int4_workspace(int64_t head_size, int64_t* bytes);
+
+/*
+ * Attention of ragged query rows over a 4-bit paged cache. Request b has queries [cum_seq_lens_q[b],
+ * cum_seq_lens_q[b + 1]) (cum_seq_lens_q NULL: query b alone, num_tokens == batch_size) and seq_lens[b]
+ * cached tokens, token i on page block_tables[b * table_stride + i / page_size], entry i % page_size. Query j of
+ * n_q sees tokens up to seq_lens[b] - n_q + j (causal), or all of them; q head h reads kv head
+ * h / (num_q_heads / num_kv_heads). out = softmax(sm_scale * q . k) v, summed in fp32 and rounded once; a query
+ * that sees no token gives zeros. lse (nullable), fp32 [num_tokens][num_q_heads]: log2 of the sum of
+ * 2^(log2(e) * sm_scale * q . k), -infinity for a query without tokens. Rows that no request covers are left as
+ * they were. Tokens of a page outside [0, num_pages) read as zeros, and lengths that do not fit num_tokens or
+ * the table are cut to them; both set MAS_STATUS_KV_SLOT_OUT_OF_RANGE. Takes the place, for a 4-bit cache, of
+ * trtllm_batch_decode_with_kv_cache / trtllm_batch_context_with_kv_cache
+ * (miniagentserve/models/devstral2/devstral2.py:184-213).
+ */
+MAS_API int mas_paged_attention_int4(const void* query, void* out, float* lse, const MasInt4KVCache* cache,
+                                     const int32_t* block_tables, int64_t table_stride, int64_t max_blocks,
+                                     const int32_t* seq_lens, const int32_t* cum_seq_lens_q, int64_t batch_size,
+                                     int64_t num_tokens, int64_t num_q_heads, int64_t num_kv_heads,
+                                     int64_t head_size, int64_t q_stride_token, int64_t q_stride_head,
+                                     int64_t out_stride_token, int64_t out_stride_head, float sm_scale, int causal,
+                                     int dtype, void* workspace, int64_t workspace_bytes, int32_t* status,
+                                     int enable_pdl, void* stream);
 
 #ifdef __cplusplus
 }

@@ -45,6 +45,14 @@ _NATIVE = {
     "read_status": ("ops", None),
     "silu_and_mul": ("ops", None),
     "silu_and_mul_quant": ("ops", None),
+    "paged_int4": ("paged_int4", None),
+    "PagedKVMaps": ("paged_int4", None),
+    "allocate_paged_kv": ("paged_int4", None),
+    "release_paged_kv": ("paged_int4", None),
+    "empty_paged_kv_cache_int4": ("paged_int4", None),
+    "append_paged_kv_cache_int4": ("paged_int4", None),
+    "read_paged_kv_cache_int4": ("paged_int4", None),
+    "paged_attention_int4": ("paged_int4", None),
 }
 # Host-only modules and names (no native library).
 _HOST = {

@@ -33,6 +33,7 @@ STATUS_EMBED_ID_OUT_OF_RANGE = 1
 STATUS_ROPE_POS_OUT_OF_RANGE = 2
 STATUS_COPY_TIMEOUT = 4
 STATUS_KV_SLOT_OUT_OF_RANGE = 8
+STATUS_KV_ALLOC_REFUSED = 16
 
 _i32, _i64, _f32, _vp = ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
 
@@ -46,6 +47,16 @@ class PagedKVCache(ctypes.Structure):
 
 
 _kvp = ctypes.POINTER(PagedKVCache)
+
+
+class Int4KVCache(ctypes.Structure):
+    """struct MasInt4KVCache (include/mas_b200.h): one layer's paged k/v cache in 4 bits."""
+
+    _fields_ = [("k_codes", _vp), ("v_codes", _vp), ("pairs", _vp), ("num_pages", _i64), ("page_size", _i64),
+                ("stride_page", _i64), ("stride_entry", _i64), ("stride_head", _i64), ("pair_stride_page", _i64)]
+
+
+_kv4p = ctypes.POINTER(Int4KVCache)
 
 # Every exported function with its argument types, in header order.
 SIGNATURES: dict[str, tuple[type, list[type]]] = {
@@ -75,6 +86,20 @@ SIGNATURES: dict[str, tuple[type, list[type]]] = {
     "mas_rope_append_paged_kv_cache": (
         _i32, [_vp, _i32, _vp, _vp, _vp, _vp, _vp, _kvp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
                _i64, _i64, _i64, _i32, _f32, _i64, _i32, _vp, _i32, _vp]),
+    "mas_allocate_paged_kv": (
+        _i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i32, _vp]),
+    "mas_release_paged_kv": (
+        _i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _i32, _vp]),
+    "mas_append_paged_kv_cache_int4": (
+        _i32, [_vp, _vp, _vp, _vp, _i32, _kv4p, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32,
+               _vp, _i32, _vp]),
+    "mas_read_paged_kv_cache_int4": (
+        _i32, [_vp, _vp, _vp, _vp, _i32, _kv4p, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32,
+               _vp, _i32, _vp]),
+    "mas_paged_attention_int4_workspace": (_i32, [_i64, ctypes.POINTER(_i64)]),
+    "mas_paged_attention_int4": (
+        _i32, [_vp, _vp, _vp, _kv4p, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+               _f32, _i32, _i32, _vp, _i64, _vp, _i32, _vp]),
 }
 
 

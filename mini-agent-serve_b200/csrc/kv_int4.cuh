@@ -1,0 +1,253 @@
+// kv_int4.cuh -- the paged KV cache held in 4 bits: its row format, the quantising append and the
+// dequantising read (sm_100a).
+//
+// A row is one token's k or v of one kv head, D values x. It is stored as D codes of 4 bits and one bf16
+// pair (scale s, minimum m):
+//   m = the largest bf16 <= min(x);   s = the smallest bf16 >= max(2^-126, (max(x) - m) / 15)
+//   c_i = floor(f32(x_i - m) / s + 1/2)   in 0..15;      value_i = c_i * s + m
+// so every x_i lies in [m, m + 15 s] and its value within s / 2 of it. The pair is bf16 because it must
+// reach as far as the activations do; rounding m down and s up, not to the nearest, keeps both ends of the row
+// inside the codes' range, at a cost of at most 2^-7 of the step. A row that holds a NaN or an infinity
+// has no such form: its pair is stored as NaN and all of it reads as NaN.
+//
+// Codes: two a byte, element 2i in the low half, k and v apart, [pages, page_size, heads, D / 2] (NHD) or
+// [pages, heads, page_size, D / 2] (HND). Pairs: bf16 [pages, heads, page_size, 4], (k s, k m, v s, v m), head-major
+// under either layout, so that a head's reader finds the pairs of consecutive tokens side by side
+// (in token-major order it would use 8 bytes of each 32-byte sector).
+//
+// The arithmetic decides every code exactly. With h = s / 2 and d = x / 2 - m / 2 (halves, so that
+// max(x) - m cannot overflow), c0 = floor(d * (1 / h)) may be one off only where d / h is nearly an integer,
+// and there both candidates round to the same code; r = fma(-(c0 + 1/2), h, d) has the sign of
+// d - (c0 + 1/2) h because that product has 13 significant bits and the fma rounds once. c = c0 + (r >= 0).
+// s is decided the same way: 15 s / 2 has 12 bits, so comparing it with the difference rounded up is exact.
+#pragma once
+
+#include <type_traits>
+
+#include "common.cuh"
+
+namespace mas {
+
+struct KVInt4Args {
+  uint8_t* k_codes;
+  uint8_t* v_codes;
+  __nv_bfloat16* pairs;
+  int64_t num_pages, page_size;
+  int64_t stride_page, stride_entry, stride_head;  // bytes; k and v codes share them
+  int64_t pair_stride_page;                        // elements
+  int32_t heads;
+};
+
+struct KVInt4RowArgs {
+  KVInt4Args kv;
+  const int32_t* kv_indices;
+  int64_t num_indices;
+  const int32_t* kv_indptr;
+  int64_t batch_size;
+  const int32_t* batch_indices;  // [T]; -1: a padding row
+  const void* pos;               // [T]
+  int64_t T;
+  void* k;  // append: the rows to store (only read); read: where they go
+  void* v;
+  int64_t ksn, ksh, vsn, vsh;  // elements
+  int32_t* status;
+};
+
+constexpr float kKVScaleMin = 1.17549435e-38f;  // 2^-126: 2 / s stays finite
+
+// The least bf16 that is >= max(2^-126, 2 * dh / 15); dh >= 0 and finite, rounded up from half the difference.
+__device__ __forceinline__ float kv_scale_up(float dh) {
+  float s = __uint_as_float(__float_as_uint(dh * (2.0f / 15.0f)) & 0xffff0000u);
+  // The truncated product is at most two bf16 steps short.
+  if (s * 7.5f < dh) s = __uint_as_float(__float_as_uint(s) + 0x10000u);
+  if (s * 7.5f < dh) s = __uint_as_float(__float_as_uint(s) + 0x10000u);
+  return fmaxf(s, kKVScaleMin);
+}
+
+// The largest bf16 that is <= x (finite).
+__device__ __forceinline__ float kv_min_down(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return __uint_as_float((u & 0xffff0000u) + ((u & 0x8000ffffu) > 0x80000000u ? 0x10000u : 0u));
+}
+
+struct KVSlot {
+  int64_t page;
+  int32_t entry;  // -1: out of range, -2: a padding row
+};
+
+template <typename PosT>
+__device__ __forceinline__ KVSlot kv_int4_slot(const KVInt4RowArgs& a, int64_t t) {
+  const int64_t b = a.batch_indices[t], pos = (int64_t)static_cast<const PosT*>(a.pos)[t];
+  if (b == -1) return {0, -2};
+  if (b < 0 || b >= a.batch_size || pos < 0) return {0, -1};
+  const int64_t first = a.kv_indptr[b];
+  const int64_t block = pos / a.kv.page_size;
+  if (first < 0 || first + block >= a.num_indices) return {0, -1};
+  const int64_t page = a.kv_indices[first + block];
+  if (page < 0 || page >= a.kv.num_pages) return {0, -1};
+  return {page, (int32_t)(pos - block * a.kv.page_size)};
+}
+
+constexpr int kKVInt4Threads = 256;
+constexpr int kKVInt4Unroll = 4;  // row pairs a warp holds at once
+
+// 8 consecutive elements of a row as four packed words.
+template <bool ALIGNED>
+__device__ __forceinline__ Vec16 kv_load8(const uint16_t* p) {
+  if (ALIGNED) return ld_ro(p);
+  Vec16 v;
+  v.a = p[0] | ((uint32_t)p[1] << 16);
+  v.b = p[2] | ((uint32_t)p[3] << 16);
+  v.c = p[4] | ((uint32_t)p[5] << 16);
+  v.d = p[6] | ((uint32_t)p[7] << 16);
+  return v;
+}
+template <bool ALIGNED>
+__device__ __forceinline__ void kv_store8(uint16_t* p, const Vec16& v) {
+  if (ALIGNED) {
+    st_plain(p, v);
+    return;
+  }
+  const uint32_t w[4] = {v.a, v.b, v.c, v.d};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    p[2 * i] = (uint16_t)w[i];
+    p[2 * i + 1] = (uint16_t)(w[i] >> 16);
+  }
+}
+
+// One pass of a warp stores 32 / (D / 8) rows (the k and the v row of one head at D = 128, of two at 64),
+// 8 elements a lane, so a row's minimum and maximum are a few shuffles away and its codes leave as one
+// 4-byte word a lane. A warp takes up to kKVInt4Unroll passes of one token, all their loads first.
+template <typename T, typename PosT, int D, bool ALIGNED>
+__global__ void __launch_bounds__(kKVInt4Threads) append_kv_int4_kernel(const KVInt4RowArgs a) {
+  constexpr int kLanes = D / 8;               // lanes a row
+  constexpr int kHeads = 32 / kLanes / 2;     // heads a pass
+  constexpr int kGroup = kHeads * kKVInt4Unroll;  // heads a warp
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int sub = lane / kLanes, col = lane % kLanes;
+  const bool is_v = sub & 1;
+  const int groups = (a.kv.heads + kGroup - 1) / kGroup;
+  const int64_t units = a.T * groups;
+  const int64_t nwarps = ((int64_t)gridDim.x * kKVInt4Threads) >> 5;
+  for (int64_t u = ((int64_t)blockIdx.x * kKVInt4Threads + threadIdx.x) >> 5; u < units; u += nwarps) {
+    const int64_t t = u / groups;
+    const int head0 = (int)(u - t * groups) * kGroup + (sub >> 1);
+    const uint16_t* row = static_cast<const uint16_t*>(is_v ? a.v : a.k) + t * (is_v ? a.vsn : a.ksn) + col * 8;
+    Vec16 x[kKVInt4Unroll];
+#pragma unroll
+    for (int i = 0; i < kKVInt4Unroll; ++i) {
+      const int h = head0 + i * kHeads;
+      if (h < a.kv.heads) x[i] = kv_load8<ALIGNED>(row + (int64_t)h * (is_v ? a.vsh : a.ksh));
+      else x[i] = Vec16{0, 0, 0, 0};
+    }
+    const KVSlot slot = kv_int4_slot<PosT>(a, t);
+    if (slot.entry < 0) {
+      if (slot.entry == -1 && lane == 0) flag_status(a.status, MAS_STATUS_KV_SLOT_OUT_OF_RANGE);
+      continue;
+    }
+    uint8_t* codes = (is_v ? a.kv.v_codes : a.kv.k_codes) + slot.page * a.kv.stride_page +
+                     slot.entry * a.kv.stride_entry + col * 4;
+    __nv_bfloat16* pairs = a.kv.pairs + slot.page * a.kv.pair_stride_page + (int64_t)slot.entry * 4 + (is_v ? 2 : 0);
+#pragma unroll
+    for (int i = 0; i < kKVInt4Unroll; ++i) {
+      const int h = head0 + i * kHeads;
+      float f[8];
+      unpack8<T>(x[i], f);
+      float lo = f[0], hi = f[0];
+      // x * 0 is NaN for a NaN or an infinity and 0 otherwise: the sum over the row tells them apart.
+      float odd = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        lo = fminf(lo, f[j]);
+        hi = fmaxf(hi, f[j]);
+        odd = fmaf(f[j], 0.0f, odd);
+      }
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) {
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        odd += __shfl_xor_sync(0xffffffffu, odd, o);
+      }
+      const bool finite = odd == 0.0f;
+      const float m = kv_min_down(lo);
+      const float nmh = -0.5f * m;
+      const float s = kv_scale_up(__fmaf_ru(hi, 0.5f, nmh));
+      const float sh = 0.5f * s, inv = __frcp_rn(sh);
+      uint32_t word = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float d = __fmaf_rn(f[j], 0.5f, nmh);
+        const float big = __fadd_rz(__fmul_rn(d, inv), 8388608.0f);  // floor, in the low bits
+        const float c0 = big - 8388608.0f;
+        const float r = fmaf(-(c0 + 0.5f), sh, d);
+        const uint32_t c = (__float_as_uint(big) & 31u) + (r >= 0.0f ? 1u : 0u);
+        word |= c << (4 * j);
+      }
+      if (h < a.kv.heads) {
+        *reinterpret_cast<uint32_t*>(codes + (int64_t)h * a.kv.stride_head) = finite ? word : 0u;
+        if (col == 0) {
+          const uint32_t pair = (__float_as_uint(s) >> 16) | (__float_as_uint(m) & 0xffff0000u);
+          *reinterpret_cast<uint32_t*>(pairs + (int64_t)h * a.kv.page_size * 4) = finite ? pair : 0x7fc07fc0u;
+        }
+      }
+    }
+  }
+  pdl_launch_dependents();
+}
+
+// A value of the cache in T: c * s + m of a row that ends near T's largest value may lie a step past it, and reads
+// as that value.
+template <typename T>
+__device__ __forceinline__ float kv_in_range(float x) {
+  const float top = Elem<T>::to_f(std::is_same<T, __half>::value ? 0x7bff : 0x7f7f);
+  x = x > top ? top : x;
+  return x < -top ? -top : x;
+}
+
+// The read-back: the same lanes, 4 bytes of codes in and 16 bytes of values out each.
+template <typename T, typename PosT, int D, bool ALIGNED>
+__global__ void __launch_bounds__(kKVInt4Threads) read_kv_int4_kernel(const KVInt4RowArgs a) {
+  constexpr int kLanes = D / 8;
+  constexpr int kHeads = 32 / kLanes / 2;
+  constexpr int kGroup = kHeads * kKVInt4Unroll;
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int sub = lane / kLanes, col = lane % kLanes;
+  const bool is_v = sub & 1;
+  const int groups = (a.kv.heads + kGroup - 1) / kGroup;
+  const int64_t units = a.T * groups;
+  const int64_t nwarps = ((int64_t)gridDim.x * kKVInt4Threads) >> 5;
+  for (int64_t u = ((int64_t)blockIdx.x * kKVInt4Threads + threadIdx.x) >> 5; u < units; u += nwarps) {
+    const int64_t t = u / groups;
+    const int head0 = (int)(u - t * groups) * kGroup + (sub >> 1);
+    const KVSlot slot = kv_int4_slot<PosT>(a, t);
+    if (slot.entry == -1 && lane == 0) flag_status(a.status, MAS_STATUS_KV_SLOT_OUT_OF_RANGE);
+    const uint8_t* codes = (is_v ? a.kv.v_codes : a.kv.k_codes) + slot.page * a.kv.stride_page +
+                           slot.entry * a.kv.stride_entry + col * 4;
+    const __nv_bfloat16* pairs = a.kv.pairs + slot.page * a.kv.pair_stride_page + (int64_t)slot.entry * 4 + (is_v ? 2 : 0);
+    uint32_t word[kKVInt4Unroll], pair[kKVInt4Unroll];
+#pragma unroll
+    for (int i = 0; i < kKVInt4Unroll; ++i) {
+      const int h = head0 + i * kHeads;
+      const bool here = slot.entry >= 0 && h < a.kv.heads;
+      word[i] = here ? *reinterpret_cast<const uint32_t*>(codes + (int64_t)h * a.kv.stride_head) : 0u;
+      pair[i] = here ? *reinterpret_cast<const uint32_t*>(pairs + (int64_t)h * a.kv.page_size * 4) : 0u;
+    }
+    uint16_t* row = static_cast<uint16_t*>(is_v ? a.v : a.k) + t * (is_v ? a.vsn : a.ksn) + col * 8;
+#pragma unroll
+    for (int i = 0; i < kKVInt4Unroll; ++i) {
+      const int h = head0 + i * kHeads;
+      if (h >= a.kv.heads) continue;
+      const float s = __uint_as_float(pair[i] << 16), m = __uint_as_float(pair[i] & 0xffff0000u);
+      float f[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = kv_in_range<T>(fmaf((float)((word[i] >> (4 * j)) & 15u), s, m));
+      kv_store8<ALIGNED>(row + (int64_t)h * (is_v ? a.vsh : a.ksh), pack8<T>(f));
+    }
+  }
+  pdl_launch_dependents();
+}
+
+}  // namespace mas

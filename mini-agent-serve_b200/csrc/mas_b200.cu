@@ -11,9 +11,12 @@
 #include <cstring>
 #include <mutex>
 
+#include "attn_int4.cuh"
 #include "common.cuh"
 #include "embed.cuh"
+#include "kv_int4.cuh"
 #include "norm.cuh"
+#include "paged_alloc.cuh"
 #include "rope.cuh"
 #include "silu.cuh"
 
@@ -31,6 +34,8 @@ constexpr int kMaxDevices = 64;
 constexpr size_t kMaxSmemPerCta = 227 * 1024;
 // Shared memory the TMA rings may use per SM: the SM has 228 KB, less 1 KB reserved per resident CTA.
 constexpr size_t kRingBytesPerSm = 216 * 1024;
+// The scanned lengths of the largest page allocation.
+constexpr size_t kAllocSmemMax = 3 * sizeof(int32_t) * (kMaxRequests + 1);
 
 struct DeviceState {
   std::once_flag once;
@@ -56,9 +61,8 @@ bool env_is(const char* name, const char* value) {
 }
 
 template <typename K>
-cudaError_t opt_in_smem(K kernel) {
-  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              (int)kMaxSmemPerCta);
+cudaError_t opt_in_smem(K kernel, size_t bytes = kMaxSmemPerCta) {
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
 }
 
 template <typename T, bool Q>
@@ -126,6 +130,14 @@ cudaError_t prepare_current(DeviceState& st, int device) {
   if ((e = opt_in_rope_ring<__half>()) != cudaSuccess) return e;
   if ((e = opt_in_smem(embed_tma_kernel<int32_t>)) != cudaSuccess) return e;
   if ((e = opt_in_smem(embed_tma_kernel<int64_t>)) != cudaSuccess) return e;
+  if ((e = opt_in_smem(paged_alloc_kernel<false, false>, kAllocSmemMax)) != cudaSuccess) return e;
+  if ((e = opt_in_smem(paged_alloc_kernel<false, true>, kAllocSmemMax)) != cudaSuccess) return e;
+  if ((e = opt_in_smem(paged_alloc_kernel<true, false>, kAllocSmemMax)) != cudaSuccess) return e;
+  if ((e = opt_in_smem(paged_alloc_kernel<true, true>, kAllocSmemMax)) != cudaSuccess) return e;
+  if ((e = opt_in_smem(attn_int4_kernel<__nv_bfloat16, 64>, AttnInt4Shape<64>::kSmem)) != cudaSuccess) return e;
+  if ((e = opt_in_smem(attn_int4_kernel<__nv_bfloat16, 128>, AttnInt4Shape<128>::kSmem)) != cudaSuccess) return e;
+  if ((e = opt_in_smem(attn_int4_kernel<__half, 64>, AttnInt4Shape<64>::kSmem)) != cudaSuccess) return e;
+  if ((e = opt_in_smem(attn_int4_kernel<__half, 128>, AttnInt4Shape<128>::kSmem)) != cudaSuccess) return e;
   void* fault = nullptr;
   if ((e = cudaGetSymbolAddress(&fault, g_fault_word)) != cudaSuccess) return e;
   st.fault = static_cast<int32_t*>(fault);
@@ -164,20 +176,30 @@ int current_device(DeviceState** out) {
 }
 
 template <typename... KArgs, typename... Args>
-int launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, void* stream, int pdl,
-           Args&&... args) {
+int launch_cluster(void (*kernel)(KArgs...), dim3 grid, dim3 block, unsigned cluster, size_t smem, void* stream,
+                   int pdl, Args&&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = pdl ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
   return e == cudaSuccess ? MAS_OK : (int)e;
+}
+
+template <typename... KArgs, typename... Args>
+int launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, void* stream, int pdl,
+           Args&&... args) {
+  return launch_cluster(kernel, grid, block, 1, smem, stream, pdl, std::forward<Args>(args)...);
 }
 
 // Resident CTAs per SM of `kernel` at this block size and dynamic shared memory, cached per
@@ -569,6 +591,126 @@ int read_word(int device, int32_t& word, int32_t* value, int clear) {
   }
   if (prev >= 0 && prev != device) (void)cudaSetDevice(prev);
   return e == cudaSuccess ? MAS_OK : (int)e;
+}
+
+// ------------------------------------------------------------------------------------------
+// The 4-bit paged cache: page allocation, append, read, attention.
+// ------------------------------------------------------------------------------------------
+template <bool RELEASE>
+int launch_alloc(AllocArgs a, int64_t outputs, DeviceState* st, void* stream, int enable_pdl) {
+  if (a.status == nullptr) a.status = st->status;
+  const size_t smem = 3 * sizeof(int32_t) * (size_t)(a.B + 1);
+  if (outputs <= kAllocSingleOutputs)
+    return launch(paged_alloc_kernel<RELEASE, false>, dim3(1), dim3(kAllocThreads), smem, stream, enable_pdl, a);
+  return launch_cluster(paged_alloc_kernel<RELEASE, true>, dim3(kAllocClusterCtas), dim3(kAllocThreads),
+                        kAllocClusterCtas, smem, stream, enable_pdl, a);
+}
+
+int make_alloc_args(AllocArgs* out, const int32_t* delta_lens, int32_t* seq_lens, int32_t* block_tables,
+                    int32_t* free_pages, int32_t* num_free, int64_t batch_size, int64_t max_blocks,
+                    int64_t table_stride, int64_t page_size, int64_t free_capacity, int32_t* status) {
+  if (batch_size < 0 || max_blocks < 0 || max_blocks > INT32_MAX || table_stride < max_blocks || page_size <= 0 ||
+      page_size > INT32_MAX || free_capacity < 0 || free_capacity > INT32_MAX || !num_free)
+    return MAS_ERR_INVALID_ARGUMENT;
+  if (batch_size > 0 && (!delta_lens || !seq_lens)) return MAS_ERR_INVALID_ARGUMENT;
+  if (batch_size > 0 && max_blocks > 0 && !block_tables) return MAS_ERR_INVALID_ARGUMENT;
+  if (free_capacity > 0 && !free_pages) return MAS_ERR_INVALID_ARGUMENT;
+  if (batch_size > kMaxRequests) return MAS_ERR_UNSUPPORTED_SHAPE;
+  AllocArgs a = {};
+  a.delta_lens = delta_lens; a.seq_lens = seq_lens; a.block_tables = block_tables; a.free_pages = free_pages;
+  a.num_free = num_free; a.table_stride = table_stride; a.free_capacity = free_capacity;
+  a.B = (int32_t)batch_size; a.max_blocks = (int32_t)max_blocks; a.page_size = (int32_t)page_size;
+  a.status = status;
+  *out = a;
+  return MAS_OK;
+}
+
+int make_int4_cache(KVInt4Args* out, const MasInt4KVCache* c, int64_t num_kv_heads, int64_t head_size) {
+  if (!c || !c->k_codes || !c->v_codes || !c->pairs || c->num_pages < 0 || c->num_pages > INT32_MAX ||
+      c->page_size <= 0 || c->page_size > INT32_MAX || num_kv_heads <= 0 || num_kv_heads > INT32_MAX ||
+      c->stride_page < 0 || c->stride_entry < 0 || c->stride_head < 0 ||
+      c->pair_stride_page < num_kv_heads * c->page_size * 4)
+    return MAS_ERR_INVALID_ARGUMENT;
+  if (head_size != 64 && head_size != 128) return MAS_ERR_UNSUPPORTED_SHAPE;
+  if (!aligned(c->k_codes, 16) || !aligned(c->v_codes, 16) || !aligned(c->pairs, 8) || c->stride_page % 16 ||
+      c->stride_entry % 16 || c->stride_head % 16 || c->pair_stride_page % 4)
+    return MAS_ERR_INVALID_ARGUMENT;
+  KVInt4Args a = {};
+  a.k_codes = static_cast<uint8_t*>(c->k_codes); a.v_codes = static_cast<uint8_t*>(c->v_codes);
+  a.pairs = static_cast<__nv_bfloat16*>(c->pairs);
+  a.num_pages = c->num_pages; a.page_size = c->page_size; a.stride_page = c->stride_page;
+  a.stride_entry = c->stride_entry; a.stride_head = c->stride_head; a.pair_stride_page = c->pair_stride_page;
+  a.heads = (int32_t)num_kv_heads;
+  *out = a;
+  return MAS_OK;
+}
+
+template <bool READ, typename T, typename PosT, int D>
+int launch_kv_int4_t(const KVInt4RowArgs& a, bool vec, DeviceState* st, void* stream, int enable_pdl) {
+  const auto kernel = READ ? (vec ? read_kv_int4_kernel<T, PosT, D, true> : read_kv_int4_kernel<T, PosT, D, false>)
+                           : (vec ? append_kv_int4_kernel<T, PosT, D, true> : append_kv_int4_kernel<T, PosT, D, false>);
+  const int64_t group = (int64_t)(256 / D / 2) * kKVInt4Unroll;  // heads a warp
+  const int64_t units = a.T * ceil_div(a.kv.heads, group);
+  const int64_t resident = (int64_t)st->sm_count * resident_ctas((const void*)kernel, kKVInt4Threads, 0);
+  const dim3 grid((unsigned)std::min(ceil_div(units, kKVInt4Threads / 32), resident));
+  return launch(kernel, grid, dim3(kKVInt4Threads), 0, stream, enable_pdl, a);
+}
+
+template <bool READ>
+int run_kv_int4(KVInt4RowArgs a, const MasInt4KVCache* cache, int64_t num_kv_heads, int64_t head_size, int dtype,
+                int positions_dtype, void* stream, int enable_pdl) {
+  if (check_act_dtype(dtype) != MAS_OK) return MAS_ERR_UNSUPPORTED_DTYPE;
+  if (positions_dtype != MAS_DTYPE_INT32 && positions_dtype != MAS_DTYPE_INT64) return MAS_ERR_UNSUPPORTED_DTYPE;
+  int rc = make_int4_cache(&a.kv, cache, num_kv_heads, head_size);
+  if (rc != MAS_OK) return rc;
+  if (a.T < 0 || a.num_indices < 0 || a.batch_size < 0 || a.ksn < 0 || a.ksh < 0 || a.vsn < 0 || a.vsh < 0)
+    return MAS_ERR_INVALID_ARGUMENT;
+  if (a.T == 0) return MAS_OK;
+  if (!a.k || !a.v || !a.batch_indices || !a.pos || !a.kv_indptr || (a.num_indices > 0 && !a.kv_indices))
+    return MAS_ERR_INVALID_ARGUMENT;
+  DeviceState* st = nullptr;
+  if ((rc = current_device(&st)) != MAS_OK) return rc;
+  if (a.status == nullptr) a.status = st->status;
+  const bool vec = aligned(a.k, 16) && aligned(a.v, 16) && a.ksn % 8 == 0 && a.ksh % 8 == 0 && a.vsn % 8 == 0 &&
+                   a.vsh % 8 == 0;
+  const bool i64 = positions_dtype == MAS_DTYPE_INT64, big = head_size == 128;
+  if (dtype == MAS_DTYPE_BF16) {
+    using T = __nv_bfloat16;
+    if (i64) return big ? launch_kv_int4_t<READ, T, int64_t, 128>(a, vec, st, stream, enable_pdl)
+                        : launch_kv_int4_t<READ, T, int64_t, 64>(a, vec, st, stream, enable_pdl);
+    return big ? launch_kv_int4_t<READ, T, int32_t, 128>(a, vec, st, stream, enable_pdl)
+               : launch_kv_int4_t<READ, T, int32_t, 64>(a, vec, st, stream, enable_pdl);
+  }
+  using T = __half;
+  if (i64) return big ? launch_kv_int4_t<READ, T, int64_t, 128>(a, vec, st, stream, enable_pdl)
+                      : launch_kv_int4_t<READ, T, int64_t, 64>(a, vec, st, stream, enable_pdl);
+  return big ? launch_kv_int4_t<READ, T, int32_t, 128>(a, vec, st, stream, enable_pdl)
+             : launch_kv_int4_t<READ, T, int32_t, 64>(a, vec, st, stream, enable_pdl);
+}
+
+// The workspace of an attention launch: every CTA's two parts, then its descriptor.
+int64_t attn_ctas(const DeviceState& st) { return (int64_t)st.sm_count * kAttnCtasPerSm; }
+int64_t attn_part_bytes(const DeviceState& st, int64_t head_size) {
+  return attn_ctas(st) * 2 * attn_part_floats((int)head_size) * (int64_t)sizeof(float);
+}
+int64_t attn_workspace_bytes(const DeviceState& st, int64_t head_size) {
+  return attn_part_bytes(st, head_size) + attn_ctas(st) * kAttnDescInts * (int64_t)sizeof(int32_t);
+}
+
+template <typename T, int D>
+int launch_attn_int4(AttnInt4Args a, DeviceState* st, void* stream, int enable_pdl) {
+  // Upper bounds on the units of work: the lengths are known to the device only.
+  const int64_t tiles = ceil_div(a.T * a.group, kAttnRows) + a.B;
+  const int64_t max_units = std::max<int64_t>(1, ceil_div((int64_t)a.max_blocks * a.kv.page_size, kAttnUnit));
+  const int64_t bound = std::min(tiles * a.kv.heads, attn_ctas(*st)) * std::min(max_units, attn_ctas(*st));
+  const unsigned grid = (unsigned)std::min(bound, attn_ctas(*st));
+  const bool split = max_units > 1;
+  if (!split) a.desc = nullptr;
+  const int rc = launch(attn_int4_kernel<T, D>, dim3(grid), dim3(kAttnThreads), AttnInt4Shape<D>::kSmem, stream,
+                        enable_pdl, a);
+  if (rc != MAS_OK || !split) return rc;
+  return launch(attn_int4_join_kernel<T, D>, dim3(grid, kAttnRows / kAttnWarps), dim3(kAttnThreads), 0, stream,
+                enable_pdl, a);
 }
 
 }  // namespace
@@ -1049,6 +1191,120 @@ int mas_embedding_gather_fill_placeholders(void* out, const void* table, void* i
   return gather_impl(out, table, ids, ids_dtype, num_tokens, hidden_size, vocab_size, out_stride,
                      table_stride, elem_size, status, enable_pdl, stream,
                      num_last > 0 ? last_tokens : nullptr, last_dtype, num_last);
+}
+
+int mas_allocate_paged_kv(const int32_t* append_lens, int32_t* seq_lens, int32_t* block_tables,
+                          const int32_t* free_pages, int32_t* num_free, int32_t* cum_lens, int32_t* batch_indices,
+                          int32_t* positions, int32_t* last_page_len, int64_t batch_size, int64_t max_blocks,
+                          int64_t table_stride, int64_t page_size, int64_t max_tokens, int64_t free_capacity,
+                          int32_t* status, int enable_pdl, void* stream) {
+  AllocArgs a;
+  int rc = make_alloc_args(&a, append_lens, seq_lens, block_tables, const_cast<int32_t*>(free_pages), num_free,
+                           batch_size, max_blocks, table_stride, page_size, free_capacity, status);
+  if (rc != MAS_OK) return rc;
+  if (max_tokens < 0 || max_tokens > INT32_MAX || !cum_lens || (batch_size > 0 && !last_page_len) ||
+      (max_tokens > 0 && (!batch_indices || !positions)))
+    return MAS_ERR_INVALID_ARGUMENT;
+  a.cum_lens = cum_lens; a.batch_indices = batch_indices; a.positions = positions; a.last_page_len = last_page_len;
+  a.max_tokens = max_tokens;
+  DeviceState* st = nullptr;
+  if ((rc = current_device(&st)) != MAS_OK) return rc;
+  return launch_alloc<false>(a, max_tokens, st, stream, enable_pdl);
+}
+
+int mas_release_paged_kv(const int32_t* keep_lens, int32_t* seq_lens, const int32_t* block_tables,
+                         int32_t* free_pages, int32_t* num_free, int64_t batch_size, int64_t max_blocks,
+                         int64_t table_stride, int64_t page_size, int64_t free_capacity, int32_t* status,
+                         int enable_pdl, void* stream) {
+  AllocArgs a;
+  int rc = make_alloc_args(&a, keep_lens, seq_lens, const_cast<int32_t*>(block_tables), free_pages, num_free,
+                           batch_size, max_blocks, table_stride, page_size, free_capacity, status);
+  if (rc != MAS_OK) return rc;
+  if (batch_size == 0) return MAS_OK;
+  DeviceState* st = nullptr;
+  if ((rc = current_device(&st)) != MAS_OK) return rc;
+  return launch_alloc<true>(a, std::min(free_capacity, batch_size * max_blocks), st, stream, enable_pdl);
+}
+
+int mas_append_paged_kv_cache_int4(const void* key, const void* value, const int32_t* batch_indices,
+                                   const void* positions, int positions_dtype, const MasInt4KVCache* cache,
+                                   const int32_t* kv_indices, int64_t num_indices, const int32_t* kv_indptr,
+                                   int64_t batch_size, int64_t num_tokens, int64_t num_kv_heads,
+                                   int64_t head_size, int64_t k_stride_token, int64_t k_stride_head,
+                                   int64_t v_stride_token, int64_t v_stride_head, int dtype, int32_t* status,
+                                   int enable_pdl, void* stream) {
+  KVInt4RowArgs a = {};
+  a.kv_indices = kv_indices; a.num_indices = num_indices; a.kv_indptr = kv_indptr; a.batch_size = batch_size;
+  a.batch_indices = batch_indices; a.pos = positions; a.T = num_tokens;
+  a.k = const_cast<void*>(key); a.v = const_cast<void*>(value);
+  a.ksn = k_stride_token; a.ksh = k_stride_head; a.vsn = v_stride_token; a.vsh = v_stride_head; a.status = status;
+  return run_kv_int4<false>(a, cache, num_kv_heads, head_size, dtype, positions_dtype, stream, enable_pdl);
+}
+
+int mas_read_paged_kv_cache_int4(void* key, void* value, const int32_t* batch_indices, const void* positions,
+                                 int positions_dtype, const MasInt4KVCache* cache, const int32_t* kv_indices,
+                                 int64_t num_indices, const int32_t* kv_indptr, int64_t batch_size,
+                                 int64_t num_tokens, int64_t num_kv_heads, int64_t head_size,
+                                 int64_t k_stride_token, int64_t k_stride_head, int64_t v_stride_token,
+                                 int64_t v_stride_head, int dtype, int32_t* status, int enable_pdl, void* stream) {
+  KVInt4RowArgs a = {};
+  a.kv_indices = kv_indices; a.num_indices = num_indices; a.kv_indptr = kv_indptr; a.batch_size = batch_size;
+  a.batch_indices = batch_indices; a.pos = positions; a.T = num_tokens; a.k = key; a.v = value;
+  a.ksn = k_stride_token; a.ksh = k_stride_head; a.vsn = v_stride_token; a.vsh = v_stride_head; a.status = status;
+  return run_kv_int4<true>(a, cache, num_kv_heads, head_size, dtype, positions_dtype, stream, enable_pdl);
+}
+
+int mas_paged_attention_int4_workspace(int64_t head_size, int64_t* bytes) {
+  if (bytes == nullptr) return MAS_ERR_INVALID_ARGUMENT;
+  if (head_size != 64 && head_size != 128) return MAS_ERR_UNSUPPORTED_SHAPE;
+  DeviceState* st = nullptr;
+  const int rc = current_device(&st);
+  if (rc != MAS_OK) return rc;
+  *bytes = attn_workspace_bytes(*st, head_size);
+  return MAS_OK;
+}
+
+int mas_paged_attention_int4(const void* query, void* out, float* lse, const MasInt4KVCache* cache,
+                             const int32_t* block_tables, int64_t table_stride, int64_t max_blocks,
+                             const int32_t* seq_lens, const int32_t* cum_seq_lens_q, int64_t batch_size,
+                             int64_t num_tokens, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_size,
+                             int64_t q_stride_token, int64_t q_stride_head, int64_t out_stride_token,
+                             int64_t out_stride_head, float sm_scale, int causal, int dtype, void* workspace,
+                             int64_t workspace_bytes, int32_t* status, int enable_pdl, void* stream) {
+  if (check_act_dtype(dtype) != MAS_OK) return MAS_ERR_UNSUPPORTED_DTYPE;
+  AttnInt4Args a = {};
+  int rc = make_int4_cache(&a.kv, cache, num_kv_heads, head_size);
+  if (rc != MAS_OK) return rc;
+  if (batch_size < 0 || batch_size > INT32_MAX || num_tokens < 0 || max_blocks < 0 || max_blocks > INT32_MAX ||
+      table_stride < max_blocks || q_stride_token < 0 || q_stride_head < 0 || out_stride_token < 0 ||
+      out_stride_head < 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads != 0 ||
+      (cum_seq_lens_q == nullptr && num_tokens != batch_size))
+    return MAS_ERR_INVALID_ARGUMENT;
+  if (num_q_heads > INT32_MAX || num_tokens > INT32_MAX / num_q_heads) return MAS_ERR_UNSUPPORTED_SHAPE;
+  if (batch_size == 0 || num_tokens == 0) return MAS_OK;
+  if (!query || !out || !seq_lens || (max_blocks > 0 && !block_tables)) return MAS_ERR_INVALID_ARGUMENT;
+  DeviceState* st = nullptr;
+  if ((rc = current_device(&st)) != MAS_OK) return rc;
+  if (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < attn_workspace_bytes(*st, head_size))
+    return MAS_ERR_INVALID_ARGUMENT;
+  a.q = query; a.out = out; a.lse = lse; a.block_tables = block_tables; a.seq_lens = seq_lens;
+  a.cum_q = cum_seq_lens_q; a.T = num_tokens; a.table_stride = table_stride; a.qsn = q_stride_token;
+  a.qsh = q_stride_head; a.osn = out_stride_token; a.osh = out_stride_head;
+  a.part = static_cast<float*>(workspace);
+  a.desc = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + attn_part_bytes(*st, head_size));
+  a.scale_log2 = sm_scale * 1.4426950408889634f;
+  a.B = (int32_t)batch_size; a.max_blocks = (int32_t)max_blocks; a.group = (int32_t)(num_q_heads / num_kv_heads);
+  a.page_shift = -1;
+  if ((a.kv.page_size & (a.kv.page_size - 1)) == 0)
+    for (a.page_shift = 0; (1ll << a.page_shift) < a.kv.page_size; ++a.page_shift) {}
+  a.causal = causal ? 1 : 0;
+  a.status = status != nullptr ? status : st->status;
+  const bool big = head_size == 128;
+  if (dtype == MAS_DTYPE_BF16)
+    return big ? launch_attn_int4<__nv_bfloat16, 128>(a, st, stream, enable_pdl)
+               : launch_attn_int4<__nv_bfloat16, 64>(a, st, stream, enable_pdl);
+  return big ? launch_attn_int4<__half, 128>(a, st, stream, enable_pdl)
+             : launch_attn_int4<__half, 64>(a, st, stream, enable_pdl);
 }
 
 }  // extern "C"

@@ -267,6 +267,185 @@ void embedding_out(at::Tensor out, at::Tensor input_ids, at::Tensor weight, bool
   gather(out, input_ids, weight, enable_pdl);
 }
 
+// ------------------------------------------------------------------------------------------------
+// The 4-bit paged cache.
+// ------------------------------------------------------------------------------------------------
+void check_int32(const at::Tensor& t, const char* name) {
+  TORCH_CHECK(t.scalar_type() == at::kInt && t.is_contiguous(), "mas_b200: ", name, " must be contiguous int32");
+}
+
+// A dimension of one entry may carry any stride: it is never stepped over.
+int64_t step_of(const at::Tensor& t, int64_t dim, int64_t otherwise) {
+  return t.size(dim) > 1 ? t.stride(dim) : otherwise;
+}
+
+MasInt4KVCache int4_cache(const at::Tensor& k_codes, const at::Tensor& v_codes, const at::Tensor& pairs, bool hnd) {
+  TORCH_CHECK(k_codes.dim() == 4 && v_codes.dim() == 4 && pairs.dim() == 4 && k_codes.sizes() == v_codes.sizes(),
+              "mas_b200: k_codes and v_codes must be 4-D with identical shapes, pairs 4-D");
+  TORCH_CHECK(k_codes.scalar_type() == at::kByte && v_codes.scalar_type() == at::kByte &&
+                  pairs.scalar_type() == at::kBFloat16,
+              "mas_b200: the codes must be uint8 and the pairs bfloat16");
+  const int64_t entries = hnd ? 2 : 1, heads = hnd ? 1 : 2;
+  MasInt4KVCache c = {};
+  c.k_codes = k_codes.data_ptr();
+  c.v_codes = v_codes.data_ptr();
+  c.pairs = pairs.data_ptr();
+  c.num_pages = k_codes.size(0);
+  c.page_size = k_codes.size(entries);
+  TORCH_CHECK(pairs.size(0) == c.num_pages && pairs.size(1) == k_codes.size(heads) && pairs.size(2) == c.page_size &&
+                  pairs.size(3) == 4,
+              "mas_b200: pairs must be (pages, heads, page_size, 4)");
+  const int64_t inner = pairs.size(2) * 4;
+  TORCH_CHECK(pairs.stride(3) == 1 && step_of(pairs, 2, 4) == 4 && step_of(pairs, 1, inner) == inner,
+              "mas_b200: pairs must be contiguous within a page");
+  c.pair_stride_page = step_of(pairs, 0, pairs.size(1) * inner);
+  TORCH_CHECK(k_codes.stride(3) == 1 && v_codes.stride(3) == 1,
+              "mas_b200: the codes' last dimension must be contiguous");
+  const int64_t row = k_codes.size(3);
+  c.stride_page = step_of(k_codes, 0, row);
+  c.stride_entry = step_of(k_codes, entries, row);
+  c.stride_head = step_of(k_codes, heads, row);
+  TORCH_CHECK(c.stride_page == step_of(v_codes, 0, row) && c.stride_entry == step_of(v_codes, entries, row) &&
+                  c.stride_head == step_of(v_codes, heads, row),
+              "mas_b200: k_codes and v_codes must have identical strides");
+  return c;
+}
+
+void allocate_paged_kv(at::Tensor append_lens, at::Tensor seq_lens, at::Tensor block_tables, at::Tensor free_pages,
+                       at::Tensor num_free, at::Tensor cum_lens, at::Tensor batch_indices, at::Tensor positions,
+                       at::Tensor last_page_len, int64_t page_size, bool enable_pdl) {
+  const c10::cuda::CUDAGuard guard(seq_lens.device());
+  const int64_t batch = seq_lens.numel();
+  check_int32(append_lens, "append_lens");
+  check_int32(seq_lens, "seq_lens");
+  check_int32(free_pages, "free_pages");
+  check_int32(num_free, "num_free");
+  check_int32(cum_lens, "cum_append_lens");
+  check_int32(batch_indices, "batch_indices");
+  check_int32(positions, "positions");
+  check_int32(last_page_len, "kv_last_page_len");
+  TORCH_CHECK(block_tables.dim() == 2 && block_tables.scalar_type() == at::kInt && block_tables.size(0) == batch &&
+                  step_of(block_tables, 1, 1) == 1,
+              "mas_b200: block_tables must be int32 (batch, max_blocks), contiguous within a row");
+  TORCH_CHECK(append_lens.numel() == batch && num_free.numel() == 1 && cum_lens.numel() == batch + 1 &&
+                  last_page_len.numel() == batch && positions.numel() == batch_indices.numel(),
+              "mas_b200: append_lens, num_free or an output has the wrong number of entries");
+  check(mas_allocate_paged_kv(append_lens.data_ptr<int32_t>(), seq_lens.data_ptr<int32_t>(),
+                              block_tables.data_ptr<int32_t>(), free_pages.data_ptr<int32_t>(),
+                              num_free.data_ptr<int32_t>(), cum_lens.data_ptr<int32_t>(),
+                              batch_indices.data_ptr<int32_t>(), positions.data_ptr<int32_t>(),
+                              last_page_len.data_ptr<int32_t>(), batch, block_tables.size(1),
+                              step_of(block_tables, 0, block_tables.size(1)), page_size, batch_indices.numel(),
+                              free_pages.numel(), nullptr, enable_pdl, stream_of(seq_lens)),
+        "mas_allocate_paged_kv");
+}
+
+void release_paged_kv(at::Tensor keep_lens, at::Tensor seq_lens, at::Tensor block_tables, at::Tensor free_pages,
+                      at::Tensor num_free, int64_t page_size, bool enable_pdl) {
+  const c10::cuda::CUDAGuard guard(seq_lens.device());
+  const int64_t batch = seq_lens.numel();
+  check_int32(keep_lens, "keep_lens");
+  check_int32(seq_lens, "seq_lens");
+  check_int32(free_pages, "free_pages");
+  check_int32(num_free, "num_free");
+  TORCH_CHECK(block_tables.dim() == 2 && block_tables.scalar_type() == at::kInt && block_tables.size(0) == batch &&
+                  step_of(block_tables, 1, 1) == 1,
+              "mas_b200: block_tables must be int32 (batch, max_blocks), contiguous within a row");
+  TORCH_CHECK(keep_lens.numel() == batch && num_free.numel() == 1,
+              "mas_b200: keep_lens or num_free has the wrong number of entries");
+  check(mas_release_paged_kv(keep_lens.data_ptr<int32_t>(), seq_lens.data_ptr<int32_t>(),
+                             block_tables.data_ptr<int32_t>(), free_pages.data_ptr<int32_t>(),
+                             num_free.data_ptr<int32_t>(), batch, block_tables.size(1),
+                             step_of(block_tables, 0, block_tables.size(1)), page_size, free_pages.numel(), nullptr,
+                             enable_pdl, stream_of(seq_lens)),
+        "mas_release_paged_kv");
+}
+
+void check_int4_rows(const at::Tensor& k, const at::Tensor& v, const at::Tensor& batch_indices,
+                     const at::Tensor& positions, const at::Tensor& k_codes, const at::Tensor& kv_indices,
+                     const at::Tensor& kv_indptr, bool hnd) {
+  TORCH_CHECK(k.dim() == 3 && v.dim() == 3 && k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type(),
+              "mas_b200: k and v must be (tokens, heads, head_size) of one dtype");
+  TORCH_CHECK(k.stride(2) == 1 && v.stride(2) == 1, "mas_b200: k and v must be contiguous in head_size");
+  check_int32(batch_indices, "batch_indices");
+  check_int32(kv_indices, "kv_indices");
+  check_int32(kv_indptr, "kv_indptr");
+  TORCH_CHECK(batch_indices.numel() == k.size(0) && positions.numel() == k.size(0) && positions.is_contiguous(),
+              "mas_b200: batch_indices and positions must be contiguous, one per token");
+  TORCH_CHECK(kv_indptr.numel() >= 1, "mas_b200: kv_indptr must have batch_size + 1 entries");
+  TORCH_CHECK(k_codes.size(hnd ? 1 : 2) == k.size(1) && 2 * k_codes.size(3) == k.size(2),
+              "mas_b200: the cache's heads/head_size differ from k's");
+}
+
+void append_paged_kv_cache_int4(at::Tensor k, at::Tensor v, at::Tensor batch_indices, at::Tensor positions,
+                                at::Tensor k_codes, at::Tensor v_codes, at::Tensor pairs, at::Tensor kv_indices,
+                                at::Tensor kv_indptr, bool hnd, bool enable_pdl) {
+  const c10::cuda::CUDAGuard guard(k.device());
+  const MasInt4KVCache c = int4_cache(k_codes, v_codes, pairs, hnd);
+  check_int4_rows(k, v, batch_indices, positions, k_codes, kv_indices, kv_indptr, hnd);
+  check(mas_append_paged_kv_cache_int4(k.data_ptr(), v.data_ptr(), batch_indices.data_ptr<int32_t>(),
+                                       positions.data_ptr(), id_code(positions), &c, kv_indices.data_ptr<int32_t>(),
+                                       kv_indices.numel(), kv_indptr.data_ptr<int32_t>(), kv_indptr.numel() - 1,
+                                       k.size(0), k.size(1), k.size(2), k.stride(0), k.stride(1), v.stride(0),
+                                       v.stride(1), act_code(k), nullptr, enable_pdl, stream_of(k)),
+        "mas_append_paged_kv_cache_int4");
+}
+
+void read_paged_kv_cache_int4(at::Tensor k, at::Tensor v, at::Tensor batch_indices, at::Tensor positions,
+                              at::Tensor k_codes, at::Tensor v_codes, at::Tensor pairs, at::Tensor kv_indices,
+                              at::Tensor kv_indptr, bool hnd, bool enable_pdl) {
+  const c10::cuda::CUDAGuard guard(k.device());
+  const MasInt4KVCache c = int4_cache(k_codes, v_codes, pairs, hnd);
+  check_int4_rows(k, v, batch_indices, positions, k_codes, kv_indices, kv_indptr, hnd);
+  check(mas_read_paged_kv_cache_int4(k.data_ptr(), v.data_ptr(), batch_indices.data_ptr<int32_t>(),
+                                     positions.data_ptr(), id_code(positions), &c, kv_indices.data_ptr<int32_t>(),
+                                     kv_indices.numel(), kv_indptr.data_ptr<int32_t>(), kv_indptr.numel() - 1,
+                                     k.size(0), k.size(1), k.size(2), k.stride(0), k.stride(1), v.stride(0),
+                                     v.stride(1), act_code(k), nullptr, enable_pdl, stream_of(k)),
+        "mas_read_paged_kv_cache_int4");
+}
+
+void paged_attention_int4(at::Tensor out, std::optional<at::Tensor> lse, at::Tensor q, at::Tensor k_codes,
+                          at::Tensor v_codes, at::Tensor pairs, at::Tensor block_tables, at::Tensor seq_lens,
+                          std::optional<at::Tensor> cum_seq_lens_q, double sm_scale, bool causal, bool hnd,
+                          bool enable_pdl) {
+  const c10::cuda::CUDAGuard guard(q.device());
+  const MasInt4KVCache c = int4_cache(k_codes, v_codes, pairs, hnd);
+  const int64_t batch = seq_lens.numel();
+  TORCH_CHECK(q.dim() == 3 && out.dim() == 3 && q.sizes() == out.sizes() && q.scalar_type() == out.scalar_type() &&
+                  q.stride(2) == 1 && out.stride(2) == 1,
+              "mas_b200: query and out must be (tokens, heads, head_size) of one dtype, contiguous within a head");
+  TORCH_CHECK(q.size(2) == 2 * k_codes.size(3), "mas_b200: the cache's head_size differs from query's");
+  check_int32(seq_lens, "seq_lens");
+  TORCH_CHECK(block_tables.dim() == 2 && block_tables.scalar_type() == at::kInt && block_tables.size(0) == batch &&
+                  step_of(block_tables, 1, 1) == 1,
+              "mas_b200: block_tables must be int32 (batch, max_blocks), contiguous within a row");
+  const int32_t* cum = nullptr;
+  if (cum_seq_lens_q.has_value()) {
+    check_int32(*cum_seq_lens_q, "cum_seq_lens_q");
+    TORCH_CHECK(cum_seq_lens_q->numel() == batch + 1, "mas_b200: cum_seq_lens_q must have batch_size + 1 entries");
+    cum = cum_seq_lens_q->data_ptr<int32_t>();
+  }
+  float* lse_ptr = nullptr;
+  if (lse.has_value()) {
+    TORCH_CHECK(lse->scalar_type() == at::kFloat && lse->is_contiguous() && lse->numel() == q.size(0) * q.size(1),
+                "mas_b200: lse must be contiguous fp32 (tokens, heads)");
+    lse_ptr = lse->data_ptr<float>();
+  }
+  if (batch == 0 || q.size(0) == 0) return;
+  // Scratch of this call alone: from the caching allocator, so a captured call keeps its own in the graph's pool.
+  int64_t bytes = 0;
+  check(mas_paged_attention_int4_workspace(q.size(2), &bytes), "mas_paged_attention_int4_workspace");
+  at::Tensor work = at::empty({bytes}, q.options().dtype(at::kByte));
+  check(mas_paged_attention_int4(q.data_ptr(), out.data_ptr(), lse_ptr, &c, block_tables.data_ptr<int32_t>(),
+                                 step_of(block_tables, 0, block_tables.size(1)), block_tables.size(1),
+                                 seq_lens.data_ptr<int32_t>(), cum, batch, q.size(0), q.size(1),
+                                 k_codes.size(hnd ? 1 : 2), q.size(2), q.stride(0), q.stride(1), out.stride(0),
+                                 out.stride(1), static_cast<float>(sm_scale), causal, act_code(q), work.data_ptr(),
+                                 bytes, nullptr, enable_pdl, stream_of(q)),
+        "mas_paged_attention_int4");
+}
+
 }  // namespace
 
 TORCH_LIBRARY(mas_b200, m) {
@@ -287,6 +466,20 @@ TORCH_LIBRARY(mas_b200, m) {
   m.def("embedding(Tensor input_ids, Tensor weight, bool enable_pdl) -> Tensor");
   m.def("embedding_out(Tensor(a!) out, Tensor input_ids, Tensor weight, bool enable_pdl) -> ()");
   m.def("embedding_fill(Tensor(a!) input_ids, Tensor weight, Tensor last_tokens, bool enable_pdl) -> Tensor");
+  m.def("allocate_paged_kv(Tensor append_lens, Tensor(a!) seq_lens, Tensor(b!) block_tables, Tensor free_pages, "
+        "Tensor(c!) num_free, Tensor(d!) cum_append_lens, Tensor(e!) batch_indices, Tensor(f!) positions, "
+        "Tensor(g!) kv_last_page_len, int page_size, bool enable_pdl) -> ()");
+  m.def("release_paged_kv(Tensor keep_lens, Tensor(a!) seq_lens, Tensor block_tables, Tensor(b!) free_pages, "
+        "Tensor(c!) num_free, int page_size, bool enable_pdl) -> ()");
+  m.def("append_paged_kv_cache_int4(Tensor k, Tensor v, Tensor batch_indices, Tensor positions, "
+        "Tensor(a!) k_codes, Tensor(b!) v_codes, Tensor(c!) pairs, Tensor kv_indices, Tensor kv_indptr, bool hnd, "
+        "bool enable_pdl) -> ()");
+  m.def("read_paged_kv_cache_int4(Tensor(a!) k, Tensor(b!) v, Tensor batch_indices, Tensor positions, "
+        "Tensor k_codes, Tensor v_codes, Tensor pairs, Tensor kv_indices, Tensor kv_indptr, bool hnd, "
+        "bool enable_pdl) -> ()");
+  m.def("paged_attention_int4(Tensor(a!) out, Tensor(b!)? lse, Tensor q, Tensor k_codes, Tensor v_codes, "
+        "Tensor pairs, Tensor block_tables, Tensor seq_lens, Tensor? cum_seq_lens_q, float sm_scale, bool causal, "
+        "bool hnd, bool enable_pdl) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(mas_b200, CUDA, m) {
@@ -301,4 +494,9 @@ TORCH_LIBRARY_IMPL(mas_b200, CUDA, m) {
   m.impl("embedding", &embedding);
   m.impl("embedding_out", &embedding_out);
   m.impl("embedding_fill", &embedding_fill);
+  m.impl("allocate_paged_kv", &allocate_paged_kv);
+  m.impl("release_paged_kv", &release_paged_kv);
+  m.impl("append_paged_kv_cache_int4", &append_paged_kv_cache_int4);
+  m.impl("read_paged_kv_cache_int4", &read_paged_kv_cache_int4);
+  m.impl("paged_attention_int4", &paged_attention_int4);
 }
