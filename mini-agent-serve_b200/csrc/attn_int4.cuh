@@ -4,21 +4,26 @@
 //   S_t = scale * (sk_t * sum_d q_d ck_td + mk_t * sum_d q_d)            (t up to the row's causal limit)
 //   o_d = (sum_t p_t sv_t (cv_td - 8) + sum_t p_t (mv_t + 8 sv_t)) / sum_t p_t,   p_t = exp(S_t - max S)
 // so the matrix products run on the bare codes, exact in 16 bits, and the pairs enter per token in fp32:
-// no key or value is ever rounded. p_t sv_t is rounded to bf16 for the second product (two bf16 terms, high and
-// low, when the queries are fp16, whose 11 bits one bf16 term would not serve); bf16 and not fp16
-// because sv_t may be anything. Maxima, sums and products are accumulated in fp32. The values' codes are centred
-// (c - 8) so that long sums do not grow one-sidedly and cancel against the minimum's part.
+// no key or value is ever rounded. The weights w_t = p_t sv_t are rounded to fp16 for the second product (11 bits
+// where bf16 has 8, whatever the queries' type); their own running reference, apart from the logits', keeps the
+// largest of a row near 1 whatever the scales are. Maxima, sums and products are accumulated in fp32. The
+// values' codes are centred (c - 8) so that long sums do not grow one-sidedly and cancel against the minima's part.
 //
 // Work split. The rows of a request that share a kv head (tokens x group, token-major) are cut into tiles of
-// 16, the tile's keys into units of 128 tokens; all units of a launch, requests outermost, form one line that the
+// 8, 16 or 32, the tile's keys into units; all units of a launch, requests outermost, form one line that the
 // CTAs cut into equal shares, whatever the lengths are (they are only known on the device). A share that
 // covers a tile's keys writes the output; the others leave (sum, maximum, unnormalised o) in the
 // workspace, and a second kernel joins them in a fixed order, so results do not change from run to run.
 //
-// A CTA is 4 warps that share the tile's queries; each takes every fourth run of 32 tokens, with a ring of
-// cp.async stages of its own, an online softmax of its own, and no barrier until the tile ends. A lane's
-// operands of mma.m16n8k16 come straight from the staged bytes: the D axis of the first product and the columns of
-// the second are permuted so that a lane's codes are 16 (8) consecutive bytes of a row.
+// A CTA is 4 warps. Where the number of kv heads is even, two take one head and two the next: under the NHD layout
+// a token's codes of two heads are one 128-byte line, and fetched apart in time they came from DRAM twice (1.085 GB
+// read for 0.572 GB at 256 requests x 2048 tokens). A head's warps take its runs of 32 tokens in turn, each with a
+// ring of cp.async stages of its own, an online softmax of its own, and no barrier until the tile ends.
+//
+// Both products have the tokens' codes as the A operand of mma.m16n8k16 (16 tokens x D, then D x 16 tokens) and
+// the rows as its 8 columns, so tiles come in steps of 8 rows and a lane's operands come straight from the
+// staged bytes: the D axis is permuted so that a lane's codes are 16 (8) consecutive bytes of a row. The weights
+// leave the first product's layout for the second's operand by one 8x8 transpose (movmatrix) each.
 #pragma once
 
 #include <type_traits>
@@ -30,11 +35,13 @@ namespace mas {
 
 constexpr int kAttnThreads = 128;
 constexpr int kAttnWarps = kAttnThreads / 32;
-constexpr int kAttnStages = 3;
-constexpr int kAttnRows = 16;
-constexpr int kAttnRun = 32;                       // tokens of one stage of one warp
-constexpr int kAttnUnit = kAttnRun * kAttnWarps;   // tokens of a unit of work
-constexpr int kAttnCtasPerSm = 4;
+constexpr int kAttnStages = 2;
+constexpr int kAttnRun = 32;  // tokens of one stage of one warp
+constexpr int kAttnMaxHeads = 2;  // kv heads a CTA takes at once
+// What starting on a tile costs (its queries, the first loads' latency, the joining of the warps), in units of work:
+// without it the shares with many short requests finish last. 256 requests of 1 to 4096 tokens, 96 / 8 heads: 310 us
+// with 0, 271 with 2, 255 with 4, 256 with 6 (before the products were all fp16).
+constexpr int kAttnLead = 4;
 
 struct AttnInt4Args {
   const void* q;
@@ -47,33 +54,44 @@ struct AttnInt4Args {
   int64_t T;
   int64_t table_stride;
   int64_t qsn, qsh, osn, osh;  // elements
-  float* part;                 // [grid][2][16 * D + 32]
-  int32_t* desc;               // [grid][kAttnDescInts]
+  float* part;                 // [grid][2][heads a CTA][rows a tile * (D + 2)]
+  int32_t* desc;               // [grid][kAttnDescInts]; nullptr: no tile can be split
   float scale_log2;            // softmax scale * log2(e)
   int32_t B, max_blocks, group;
   int32_t page_shift;          // log2(page_size), or -1
   int32_t causal;
+  int32_t cta_heads;           // 1 or 2
+  int32_t q_vec;               // rows of queries are 16-byte aligned
+  uint32_t page16, entry16;    // the codes' strides in units of 16 bytes
   int32_t* status;
 };
 
 // What the joining kernel needs of a tile that was split: written by the CTA whose share starts the tile.
-// {number of parts (0: nothing to join), request, the tile's first row within it, kv head}
+// {number of parts (0: nothing to join), request, the tile's first row within it, first kv head}
 constexpr int kAttnDescInts = 4;
 
-__host__ __device__ constexpr int attn_part_floats(int D) { return kAttnRows * D + 2 * kAttnRows; }
+// NT: the tile's rows in eights.
+__host__ __device__ constexpr int attn_part_floats(int D, int NT) { return 8 * NT * (D + 2); }
 
-template <int D>
+template <int D, int NT>
 struct AttnInt4Shape {
+  static constexpr int kRows = 8 * NT;
+  static constexpr int kPass = NT == 4 ? 1 : 2;  // 16-token steps a warp computes at once
+  // By registers (128, 168 and 255 a thread). At 16 rows four CTAs of 128 registers took 211 us where three take 196
+  // (spills, or half the independent products a warp), two of 255 took 221.
+  static constexpr int kCtasPerSm = NT == 1 ? 4 : NT == 2 ? 3 : 2;
   static constexpr int kRowBytes = D / 2;
   static constexpr int kKeys = 0;
   static constexpr int kValues = kAttnRun * kRowBytes;
   static constexpr int kPairs = 2 * kAttnRun * kRowBytes;
-  static constexpr int kStage = kPairs + kAttnRun * 8;
+  static constexpr int kFactors = kPairs + kAttnRun * 8;         // the pairs as fp32 factors
+  static constexpr int kStage = kFactors + kAttnRun * 16;
   static constexpr int kWarpRing = kAttnStages * kStage;
-  static constexpr int kQFrag = D / 16 * 32 * 16;
-  static constexpr int kMerge = kAttnWarps * (D / 2) * 32 * 4;  // the warps' o; their statistics follow
+  static constexpr int kQHead = D / 32 * NT * 512;               // a head's queries as operands
+  static constexpr int kQFrag = kAttnMaxHeads * kQHead;
+  static constexpr int kMerge = kAttnWarps * (D / 4 * NT) * 32 * 4;  // the warps' o
   static constexpr int kRing = kAttnWarps * kWarpRing;
-  static constexpr int kStats = kAttnWarps * kAttnRows * 2 * 4;
+  static constexpr int kStats = kAttnWarps * kRows * 3 * 4;
   static constexpr int kSmem = kQFrag + (kRing > kMerge ? kRing : kMerge) + kStats;
 };
 
@@ -84,6 +102,9 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool v
 __device__ __forceinline__ void cp_async8(uint32_t dst, const void* src, bool valid) {
   const int bytes = valid ? 8 : 0;
   asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -101,35 +122,34 @@ __device__ __forceinline__ uint2 lds64(uint32_t a) {
   asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
   return v;
 }
+__device__ __forceinline__ void sts128(uint32_t a, float x, float y, float z, float w) {
+  asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(a), "f"(x), "f"(y), "f"(z), "f"(w) : "memory");
+}
+__device__ __forceinline__ float2 lds_float2(uint32_t a) {
+  const uint2 v = lds64(a);
+  return make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
+}
 __device__ __forceinline__ uint32_t lds32(uint32_t a) {
   uint32_t v;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
   return v;
 }
 
-__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                         uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-      "{%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma_fp16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                         uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-      "{%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-// (w & mask) | magic in one instruction.
-__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t magic) {
-  uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "r"(mask), "r"(magic));
-  return r;
-}
+#define MAS_MMA(NAME, SHAPE)                                                                                     \
+  __device__ __forceinline__ void NAME(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,         \
+                                       uint32_t b0, uint32_t b1) {                                               \
+    asm volatile("mma.sync.aligned." SHAPE " {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"     \
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])                                                \
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));                                        \
+  }                                                                                                              \
+  __device__ __forceinline__ void NAME##_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, \
+                                               uint32_t b0, uint32_t b1) {                                       \
+    asm volatile("mma.sync.aligned." SHAPE " {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};" \
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])                                                \
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));                             \
+  }
+MAS_MMA(mma_fp16, "m16n8k16.row.col.f32.f16.f16.f32")
+#undef MAS_MMA
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -137,66 +157,64 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// The key codes of a word as 16-bit pairs (e0, e4), (e1, e5), (e2, e6), (e3, e7). bf16: 128 + c (the bias
-// leaves with the sum of q, in the accumulator's start value); fp16: c - 8.
-template <typename T>
-struct KeyCodes;
-template <>
-struct KeyCodes<__nv_bfloat16> {
-  static constexpr float kStart = -128.0f;  // accumulators start at this times sum q
-  static constexpr float kCentre = 0.0f;    // a product is sum q (c - kCentre)
-  static __device__ __forceinline__ void unpack(uint32_t w, uint32_t (&p)[4]) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) p[i] = and_or(w >> (4 * i), 0x000f000fu, 0x43004300u);
-  }
-  static __device__ __forceinline__ void mma(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
-    mma_bf16(c, a.x, a.y, a.z, a.w, b0, b1);
-  }
-};
-template <>
-struct KeyCodes<__half> {
-  static constexpr float kStart = 0.0f;
-  static constexpr float kCentre = 8.0f;
-  static __device__ __forceinline__ void unpack(uint32_t w, uint32_t (&p)[4]) {
-    const __half2 off = __floats2half2_rn(1032.0f, 1032.0f), sixteenth = __floats2half2_rn(0.0625f, 0.0625f);
-    const __half2 off16 = __floats2half2_rn(-72.0f, -72.0f);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      uint32_t lo = and_or(w >> (8 * i), 0x000f000fu, 0x64006400u);  // 1024 + c
-      uint32_t hi = and_or(w >> (8 * i), 0x00f000f0u, 0x64006400u);  // 1024 + 16 c
-      __half2 x = __hsub2(*reinterpret_cast<__half2*>(&lo), off);
-      __half2 y = __hfma2(*reinterpret_cast<__half2*>(&hi), sixteenth, off16);
-      p[2 * i] = *reinterpret_cast<uint32_t*>(&x);
-      p[2 * i + 1] = *reinterpret_cast<uint32_t*>(&y);
-    }
-  }
-  static __device__ __forceinline__ void mma(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
-    mma_fp16(c, a.x, a.y, a.z, a.w, b0, b1);
-  }
-};
-
-// Code pair i of a word whose halves hold two tokens' codes, as bf16 c - 8 (exact).
-__device__ __forceinline__ uint32_t value_codes(uint32_t x, int i) {
-  uint32_t u = and_or(x >> (4 * i), 0x000f000fu, 0x43004300u);  // 128 + c
-  const __nv_bfloat162 off = __floats2bfloat162_rn(136.0f, 136.0f);
-  __nv_bfloat162 y = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&u), off);
-  return *reinterpret_cast<uint32_t*>(&y);
+// A code word's nibbles at bits 0, 4, 8, 12 of each half as fp16 pairs. A nibble c at the foot of a half IS the
+// fp16 denormal c * 2^-24, one nibble up c * 2^-20: two masks a byte, no arithmetic.
+constexpr float kEvenUnit = 16777216.0f, kOddUnit = 1048576.0f;  // 2^24, 2^20: what undoes that
+__device__ __forceinline__ void nibbles_fp16(uint32_t w, uint32_t (&p)[4]) {
+  p[0] = w & 0x000f000fu;
+  p[1] = w & 0x00f000f0u;
+  p[2] = (w >> 8) & 0x000f000fu;
+  p[3] = (w >> 8) & 0x00f000f0u;
 }
 
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-  return Elem<__nv_bfloat16>::from_f2(lo, hi);
+// One lane's 8 query elements that meet one code word, as the first product's operand: elements that meet odd
+// nibbles are divided by 16. bf16 rows are first scaled by a power of two to a largest element of 2^11 to 2^12, where fp16
+// holds their 8 bits down to 2^-25 of that largest; fp16 rows are taken as they are (an odd element below 2^-10 loses bits
+// past 2^-21).
+__device__ __forceinline__ uint4 query_operand(const float (&f)[8], float scale) {
+  const float odd = scale * 0.0625f;
+  return make_uint4(Elem<__half>::from_f2(f[0] * scale, f[4] * scale), Elem<__half>::from_f2(f[1] * odd, f[5] * odd),
+                    Elem<__half>::from_f2(f[2] * scale, f[6] * scale), Elem<__half>::from_f2(f[3] * odd, f[7] * odd));
 }
 
-// Where a staged value row's 16-byte chunk lies: rows are reordered (and at D = 128 chunks exchanged) so that the
-// four rows 2t (or 2t + 1) that a warp reads at once fall into different banks.
+// The 8x8 matrix of 16-bit elements held as pairs (row lane / 4, columns 2 (lane % 4), + 1), transposed.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+__device__ __forceinline__ float2 add2_f32(float2 a, float2 b) {
+  float2 c;
+  asm("{\n\t.reg .b64 ra, rb, rc;\n\t"
+      "mov.b64 ra, {%2, %3};\n\t"
+      "mov.b64 rb, {%4, %5};\n\t"
+      "add.rn.f32x2 rc, ra, rb;\n\t"
+      "mov.b64 {%0, %1}, rc;\n\t}"
+      : "=f"(c.x), "=f"(c.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return c;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ uint32_t max_nan_half2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// Where a staged value row's 16-byte chunk lies: exchanged so that one chunk of eight consecutive rows, which a matrix
+// load reads at once, covers all banks.
 template <int D>
-__device__ __forceinline__ uint32_t value_offset(int row, int byte) {
-  if (D == 128) {
-    const int phys = (row & ~3) | ((row & 1) << 1) | ((row >> 1) & 1);
-    return phys * 64 + (byte ^ (((row >> 2) & 1) << 5));
-  }
-  const int phys = (row & ~7) | ((row & 1) << 2) | ((row >> 1) & 3);
-  return phys * 32 + byte;
+__device__ __forceinline__ uint32_t value_offset(int row, int chunk) {
+  return D == 128 ? row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4) : row * 32 + ((chunk ^ ((row >> 2) & 1)) << 4);
+}
+
+// Four 8x8 matrices of 16-bit units, transposed: matrix i's rows are the 16 bytes at lanes 8i .. 8i + 7's addresses; lane
+// (g, t) receives column g of rows 2t, 2t + 1 of each.
+__device__ __forceinline__ void load_transposed(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a));
 }
 
 // A request's extent, with every length that does not fit its buffers cut to them.
@@ -204,17 +222,19 @@ struct AttnRequest {
   int32_t q0, qlen;  // first query row, queries
   int32_t n;         // tokens in the cache
   int32_t tiles, units;
-  __device__ __forceinline__ int64_t work(int heads) const { return (int64_t)tiles * heads * units; }
+  __device__ __forceinline__ int64_t work(int head_groups) const { return (int64_t)tiles * head_groups * (units + kAttnLead); }
 };
 
+template <int ROWS>
 __device__ __forceinline__ AttnRequest attn_request(const AttnInt4Args& a, int b, int32_t* status) {
+  const int unit = kAttnRun * (kAttnWarps / a.cta_heads);
   AttnRequest r;
   int64_t q0 = b, q1 = b + 1;
   if (a.cum_q != nullptr) {
     q0 = a.cum_q[b];
     q1 = a.cum_q[b + 1];
   }
-  const int64_t capacity = min((int64_t)a.max_blocks * a.kv.page_size, (int64_t)INT32_MAX - kAttnUnit);
+  const int64_t capacity = min((int64_t)a.max_blocks * a.kv.page_size, (int64_t)INT32_MAX - 2 * kAttnRun * kAttnWarps);
   int64_t n = a.seq_lens[b];
   if (q0 < 0 || q1 < q0 || q1 > a.T || n < 0 || n > capacity) {
     flag_status(status, MAS_STATUS_KV_SLOT_OUT_OF_RANGE);
@@ -225,36 +245,46 @@ __device__ __forceinline__ AttnRequest attn_request(const AttnInt4Args& a, int b
   r.q0 = (int32_t)q0;
   r.qlen = (int32_t)(q1 - q0);
   r.n = (int32_t)n;
-  r.tiles = (int32_t)(((int64_t)r.qlen * a.group + kAttnRows - 1) / kAttnRows);
-  r.units = max(1, (r.n + kAttnUnit - 1) / kAttnUnit);
+  r.tiles = (int32_t)(((int64_t)r.qlen * a.group + ROWS - 1) / ROWS);
+  r.units = max(1, (r.n + unit - 1) / unit);
   return r;
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kAttnThreads, kAttnCtasPerSm) attn_int4_kernel(const AttnInt4Args a) {
-  using Sh = AttnInt4Shape<D>;
-  using Keys = KeyCodes<T>;
-  constexpr int kNt = D / 8;        // column tiles of the second product
-  constexpr int kWords = D / 32;    // key words a lane and token
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kAttnThreads, AttnInt4Shape<D, NT>::kCtasPerSm)
+    attn_int4_kernel(const AttnInt4Args a) {
+  using Sh = AttnInt4Shape<D, NT>;
+  constexpr bool kRowScale = std::is_same<T, __nv_bfloat16>::value;
+  // fp16 results: the second product's codes are centred (c - 7.5), through one more product with ones that sums the
+  // rounded weights; their rounding then meets codes of half the size. bf16 results are rounded 8 times coarser.
+  constexpr bool kCentred = std::is_same<T, __half>::value;
+  constexpr float kCentre = kCentred ? 7.5f : 0.0f;
+  constexpr int kRows = Sh::kRows;
+  constexpr int kMt = D / 16;     // 16-row tiles of the second product's D axis
+  constexpr int kWords = D / 32;  // key code words a lane and token
+  constexpr int kPass = Sh::kPass;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int64_t s_scan[kAttnWarps + 2];
   __shared__ int32_t s_b;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
   uint8_t* ring = smem + Sh::kQFrag;
-  const uint32_t qfrag_u = smem_u32(smem);
   const uint32_t ring_u = smem_u32(ring) + warp * Sh::kWarpRing;
   float* merge = reinterpret_cast<float*>(ring);
-  float* stats = reinterpret_cast<float*>(smem + Sh::kSmem - Sh::kStats);  // [warp][row][max, sum]
+  float* stats = reinterpret_cast<float*>(smem + Sh::kSmem - Sh::kStats);  // [warp][row][m, l]
+  float* qrow = stats + kAttnWarps * kRows * 2;                            // [head][pair of rows][2 sums of q, 2 scales]
   int32_t* desc = a.desc + (int64_t)blockIdx.x * kAttnDescInts;
   pdl_wait();
 
   // This CTA's share of the line of units: total by a block sum, the request it starts in by the scan.
-  const int heads = a.kv.heads;
+  const int cta_heads = a.cta_heads, head_warps = kAttnWarps / cta_heads, head_groups = a.kv.heads / cta_heads;
+  const int unit_tokens = kAttnRun * head_warps;
+  const int which = warp / head_warps, sub_warp = warp % head_warps;  // this warp's head of the CTA's, its place there
   const int per = (a.B + kAttnThreads - 1) / kAttnThreads;
   const int rb0 = min(a.B, tid * per), rb1 = min(a.B, rb0 + per);
   int64_t mine = 0;
-  for (int b = rb0; b < rb1; ++b) mine += attn_request(a, b, blockIdx.x == 0 ? a.status : nullptr).work(heads);
+  for (int b = rb0; b < rb1; ++b)
+    mine += attn_request<kRows>(a, b, blockIdx.x == 0 ? a.status : nullptr).work(head_groups);
   int64_t incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -281,7 +311,7 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtasPerSm) attn_int4_kernel
     int64_t rem = at - before;
     int b = rb0;
     for (; b < rb1; ++b) {
-      const int64_t w = attn_request(a, b, nullptr).work(heads);
+      const int64_t w = attn_request<kRows>(a, b, nullptr).work(head_groups);
       if (rem < w) break;
       rem -= w;
     }
@@ -290,58 +320,82 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtasPerSm) attn_int4_kernel
   }
   __syncthreads();
   int b = s_b;
-  AttnRequest rq = attn_request(a, b, nullptr);
-  int unit, head, tile;
+  AttnRequest rq = attn_request<kRows>(a, b, nullptr);
+  int unit, head_group, tile;
   {
     int64_t rem = s_scan[kAttnWarps];
-    unit = (int)(rem % rq.units);
-    rem /= rq.units;
-    head = (int)(rem % heads);
-    tile = (int)(rem / heads);
+    unit = (int)(rem % (rq.units + kAttnLead)) - kAttnLead;  // below 0: the start's cost
+    rem /= rq.units + kAttnLead;
+    head_group = (int)(rem % head_groups);
+    tile = (int)(rem / head_groups);
   }
   int desc_parts = 0, desc_request = 0, desc_row = 0, desc_head = 0;
 
   while (at < end) {
+    // Of this share, the start's cost is passed over. A share may hold nothing but (a part of) that.
+    const int lead = (int)min((int64_t)max(-unit, 0), end - at);
+    at += lead;
+    unit += lead;
+    if (at == end) break;
     const int seg_units = (int)min((int64_t)(rq.units - unit), end - at);
-    const int rows_here = min(kAttnRows, rq.qlen * a.group - tile * kAttnRows);
-    const int row0 = tile * kAttnRows;
-    // Keys visible to a row: those before its limit. Rows past the tile's last take the last one's limit.
-    const int last_tok = (row0 + rows_here - 1) / a.group;
-    const int tile_end = a.causal ? min(rq.n, max(0, rq.n - rq.qlen + last_tok + 1)) : rq.n;
-    const int t0 = unit * kAttnUnit;
-    const int t1 = min((unit + seg_units) * kAttnUnit, tile_end);
-    int lim0 = tile_end, lim1 = tile_end, lim_first = tile_end;
-    if (a.causal) {
-      lim_first = max(0, rq.n - rq.qlen + row0 / a.group + 1);
-      if (g < rows_here) lim0 = max(0, rq.n - rq.qlen + (row0 + g) / a.group + 1);
-      if (g + 8 < rows_here) lim1 = max(0, rq.n - rq.qlen + (row0 + g + 8) / a.group + 1);
-    }
+    const int row0 = tile * kRows;
+    const int rows_here = min(kRows, rq.qlen * a.group - row0);
+    const int head = head_group * cta_heads + which;
+    // Tokens visible to row r of the tile: those before its limit. Rows past the last take the last one's limit.
+    auto limit = [&](int r) {
+      const int tok = (row0 + min(r, rows_here - 1)) / a.group;
+      return a.causal ? min(rq.n, max(0, rq.n - rq.qlen + tok + 1)) : rq.n;
+    };
+    const int t0 = unit * unit_tokens;
+    const int t1 = min((unit + seg_units) * unit_tokens, limit(kRows - 1));
+    const int lim_first = limit(0);
+    const uint32_t head16 = (uint32_t)(head * a.kv.stride_head >> 4);
 
-    // Queries into shared memory in the order the first product takes them: k step 2i of lane (g, t) holds
-    // elements 0, 4 and 1, 5 of 32-bit code word i of the lane's stretch of the row, step 2i + 1 the rest.
-    for (int e = tid; e < D / 16 * 32; e += kAttnThreads) {
-      const int step = e >> 5, l = e & 31;
-      const int d = (D / 4) * (l & 3) + 8 * (step >> 1) + 2 * (step & 1);
-      uint32_t v[4];
+    // Queries into shared memory as the first product takes them, a warp for eight rows of a head: lane (g, t) has
+    // elements (D / 4) t and on of row g. Beside them the rows' sums and scales, two rows (2t, 2t + 1) together.
+    for (int c = warp; c < cta_heads * NT; c += kAttnWarps) {
+      const int nt = c % NT, hd = c / NT, rr = nt * 8 + g;
+      float f[D / 32][8], sum = 0.0f, most = 0.0f;
+      const int tok = (row0 + min(rr, rows_here - 1)) / a.group, sub = row0 + min(rr, rows_here - 1) - tok * a.group;
+      const uint16_t* src = static_cast<const uint16_t*>(a.q) + (int64_t)(rq.q0 + tok) * a.qsn +
+                            ((int64_t)(head_group * cta_heads + hd) * a.group + sub) * a.qsh + (D / 4) * t;
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int r = row0 + (l >> 2) + 8 * half;
-        const bool here = (l >> 2) + 8 * half < rows_here;
-        const int tok = r / a.group, sub = r - tok * a.group;
-        const uint16_t* src = static_cast<const uint16_t*>(a.q) + (int64_t)(rq.q0 + tok) * a.qsn +
-                              ((int64_t)head * a.group + sub) * a.qsh + d;
-        v[half] = here ? src[0] | ((uint32_t)src[4] << 16) : 0u;
-        v[2 + half] = here ? src[1] | ((uint32_t)src[5] << 16) : 0u;
+      for (int i = 0; i < D / 32; ++i) {
+        unpack8<T>(a.q_vec ? kv_load8<true>(src + 8 * i) : kv_load8<false>(src + 8 * i), f[i]);
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          f[i][x] = rr < rows_here ? f[i][x] : 0.0f;
+          sum += f[i][x];
+          // as bits, so that a NaN is the most
+          most = __uint_as_float(max(__float_as_uint(most), __float_as_uint(fabsf(f[i][x]))));
+        }
       }
-      *reinterpret_cast<uint4*>(smem + e * 16) = make_uint4(v[0], v[1], v[2], v[3]);
+#pragma unroll
+      for (int z = 1; z < 4; z <<= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, z);
+        most = __uint_as_float(max(__float_as_uint(most), __shfl_xor_sync(0xffffffffu, __float_as_uint(most), z)));
+      }
+      const uint32_t exponent = min(max(__float_as_uint(most) >> 23, 12u), 254u);
+      const float scale = kRowScale ? __uint_as_float((265u - exponent) << 23) : 1.0f;
+      const float unscale = kRowScale ? __uint_as_float((exponent - 11u) << 23) : 1.0f;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+        *reinterpret_cast<uint4*>(smem + hd * Sh::kQHead + ((i * NT + nt) * 32 + lane) * 16) =
+            query_operand(f[i], scale);
+      if (t == 0) {
+        float* dst = qrow + (hd * kRows + nt * 8 + (g & ~1)) * 2 + (g & 1);
+        dst[0] = sum * scale;
+        dst[2] = unscale;
+      }
     }
+    const uint32_t qfrag_u = smem_u32(smem) + which * Sh::kQHead + lane * 16;
 
-    // The warp's runs: t0 + 32 (warp + 4 i).
+    // The warp's runs: t0 + 32 (sub_warp + head_warps * i).
     const int runs_all = t1 > t0 ? (t1 - t0 + kAttnRun - 1) / kAttnRun : 0;
-    const int runs = runs_all > warp ? (runs_all - warp + kAttnWarps - 1) / kAttnWarps : 0;
+    const int runs = runs_all > sub_warp ? (runs_all - sub_warp + head_warps - 1) / head_warps : 0;
     const int32_t* table = a.block_tables + (int64_t)b * a.table_stride;
     auto load_page = [&](int i) {
-      const int tok = t0 + kAttnRun * (warp + kAttnWarps * i) + lane;
+      const int tok = t0 + kAttnRun * (sub_warp + head_warps * i) + lane;
       if (i >= runs || tok >= t1) return -1;
       const int block = a.page_shift >= 0 ? tok >> a.page_shift : tok / (int)a.kv.page_size;
       const int page = table[block];  // block < max_blocks: tok < n <= capacity
@@ -351,24 +405,31 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtasPerSm) attn_int4_kernel
       }
       return page;
     };
+    // Offsets travel in units of 16 bytes: 32 bits reach 64 GB (checked by the host).
     auto issue = [&](int i, int page) {
       if (i < runs) {
-        const int tok = t0 + kAttnRun * (warp + kAttnWarps * i) + lane;
+        const int tok = t0 + kAttnRun * (sub_warp + head_warps * i) + lane;
         const int entry = a.page_shift >= 0 ? tok & ((1 << a.page_shift) - 1) : tok % (int)a.kv.page_size;
         const uint32_t stage = ring_u + (i % kAttnStages) * Sh::kStage;
-        int64_t off = -1;
-        if (page >= 0)
-          off = page * a.kv.stride_page + entry * a.kv.stride_entry + head * a.kv.stride_head;
+        const uint32_t valid = __ballot_sync(0xffffffffu, page >= 0);
+        const uint32_t off = page >= 0 ? (uint32_t)page * a.page16 + (uint32_t)entry * a.entry16 + head16 : 0u;
         constexpr int kChunks = Sh::kRowBytes / 16;
         constexpr int kRowsAtOnce = 32 / kChunks;
+        const int chunk = lane % kChunks;
 #pragma unroll
         for (int it = 0; it < kAttnRun / kRowsAtOnce; ++it) {
-          const int row = it * kRowsAtOnce + lane / kChunks, byte = lane % kChunks * 16;
-          const int64_t o = __shfl_sync(0xffffffffu, off, row);
-          const bool ok = o >= 0;
-          const int64_t src = ok ? o + byte : 0;
-          cp_async16(stage + Sh::kKeys + row * Sh::kRowBytes + byte, a.kv.k_codes + src, ok);
-          cp_async16(stage + Sh::kValues + value_offset<D>(row, byte), a.kv.v_codes + src, ok);
+          const int row = it * kRowsAtOnce + lane / kChunks;
+          const uint64_t src = (uint64_t)(__shfl_sync(0xffffffffu, off, row) + chunk) * 16;
+          const uint32_t to_k = stage + Sh::kKeys + row * Sh::kRowBytes + chunk * 16;
+          const uint32_t to_v = stage + Sh::kValues + value_offset<D>(row, chunk);
+          if (valid == 0xffffffffu) {
+            cp_async16(to_k, a.kv.k_codes + src);
+            cp_async16(to_v, a.kv.v_codes + src);
+          } else {
+            const bool ok = (valid >> row) & 1u;
+            cp_async16(to_k, a.kv.k_codes + src, ok);
+            cp_async16(to_v, a.kv.v_codes + src, ok);
+          }
         }
         const int64_t pair = page >= 0 ? page * a.kv.pair_stride_page + ((int64_t)head * a.kv.page_size + entry) * 4 : 0;
         cp_async8(stage + Sh::kPairs + lane * 8, a.kv.pairs + pair, page >= 0);
@@ -384,25 +445,258 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtasPerSm) attn_int4_kernel
     }
     __syncthreads();  // the queries are in shared memory
 
-    float qsum0 = 0.0f, qsum1 = 0.0f;
-#pragma unroll
-    for (int s = 0; s < D / 16; ++s) {
-      const uint4 v = lds128(qfrag_u + (s * 32 + lane) * 16);
-      const float2 x = Elem<T>::to_f2(v.x), y = Elem<T>::to_f2(v.y), z = Elem<T>::to_f2(v.z), w = Elem<T>::to_f2(v.w);
-      qsum0 += (x.x + x.y) + (z.x + z.y);
-      qsum1 += (y.x + y.y) + (w.x + w.y);
-    }
-    qsum0 += __shfl_xor_sync(0xffffffffu, qsum0, 1);
-    qsum0 += __shfl_xor_sync(0xffffffffu, qsum0, 2);
-    qsum1 += __shfl_xor_sync(0xffffffffu, qsum1, 1);
-    qsum1 += __shfl_xor_sync(0xffffffffu, qsum1, 2);
+    const uint32_t qrow_u = smem_u32(qrow) + which * kRows * 8 + t * 16;
 
-    float o[kNt][4];
+    // o: tile j of the D axis holds elements 32 (j / 2) + 4g + 2 (j % 2) and the next, of rows 2t, 2t + 1. l and r (the
+    // minima's part) are relative to 2^-nref, o to 2^-nref / wscale, wscale a power of two; l == 0: the row has seen no key
+    // and nref means nothing.
+    float o[kMt][NT][4];
+    float2 nref[NT], wscale[NT], l[NT], r[NT];
+    float wsum[kCentred ? NT : 1][4];  // the sum of the rounded weights, of rows 2t, 2t + 1 (twice)
 #pragma unroll
-    for (int j = 0; j < kNt; ++j)
+    for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) o[j][c] = 0.0f;
-    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f, r0 = 0.0f, r1 = 0.0f;
+      for (int j = 0; j < kMt; ++j)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[j][nt][c] = 0.0f;
+      wscale[nt] = both(1.0f);
+      nref[nt] = l[nt] = r[nt] = both(0.0f);
+      if (kCentred) wsum[nt][0] = wsum[nt][1] = wsum[nt][2] = wsum[nt][3] = 0.0f;
+    }
+
+    // Run i has landed: each lane turns its token's pairs into what the logits (in units of log2) and the values need.
+    auto make_factors = [&](int i) {
+      const uint32_t stage = ring_u + (i % kAttnStages) * Sh::kStage;
+      const uint2 pr = lds64(stage + Sh::kPairs + lane * 8);
+      const float sk = __uint_as_float(pr.x << 16), km = __uint_as_float(pr.x & 0xffff0000u);
+      const float sv = __uint_as_float(pr.y << 16), vm = __uint_as_float(pr.y & 0xffff0000u);
+      sts128(stage + Sh::kFactors + lane * 16, sk * (a.scale_log2 * kEvenUnit), km * a.scale_log2, sv,
+             fmaf(kCentre, sv, vm));
+      __syncwarp();
+    };
+    // The first product and the keys' pairs: the logits (over the row's scale) of kPass 16-token steps from p0 on,
+    // s[x][nt] = tokens g, g + 8 of step p0 + x, rows 2t, 2t + 1.
+    auto logits = [&](int i, int p0, float (&s)[kPass][NT][4]) {
+      const uint32_t stage = ring_u + (i % kAttnStages) * Sh::kStage;
+      uint32_t kw[kPass][2][kWords];
+#pragma unroll
+      for (int x = 0; x < kPass; ++x)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const uint32_t at_row = stage + Sh::kKeys + ((p0 + x) * 16 + half * 8 + g) * Sh::kRowBytes + t * (D / 8);
+          if (D == 128) {
+            const uint4 v = lds128(at_row);
+            kw[x][half][0] = v.x; kw[x][half][1] = v.y;
+            kw[x][half][kWords - 2] = v.z; kw[x][half][kWords - 1] = v.w;
+          } else {
+            const uint2 v = lds64(at_row);
+            kw[x][half][0] = v.x; kw[x][half][1] = v.y;
+          }
+        }
+#pragma unroll
+      for (int w = 0; w < kWords; ++w) {
+        uint32_t ka[kPass][2][4];
+#pragma unroll
+        for (int x = 0; x < kPass; ++x)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) nibbles_fp16(kw[x][half][w], ka[x][half]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const uint4 qb = lds128(qfrag_u + (w * NT + nt) * 512);
+#pragma unroll
+          for (int x = 0; x < kPass; ++x) {
+            if (w == 0) mma_fp16_first(s[x][nt], ka[x][0][0], ka[x][1][0], ka[x][0][1], ka[x][1][1], qb.x, qb.y);
+            else mma_fp16(s[x][nt], ka[x][0][0], ka[x][1][0], ka[x][0][1], ka[x][1][1], qb.x, qb.y);
+            mma_fp16(s[x][nt], ka[x][0][2], ka[x][1][2], ka[x][0][3], ka[x][1][3], qb.z, qb.w);
+          }
+        }
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float2 qs = lds_float2(qrow_u + nt * 64);
+#pragma unroll
+        for (int x = 0; x < kPass; ++x)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const float2 f = lds_float2(stage + Sh::kFactors + ((p0 + x) * 16 + half * 8 + g) * 16);
+            const float2 y = fma2_f32(make_float2(s[x][nt][2 * half], s[x][nt][2 * half + 1]), both(f.x), mul2_f32(qs, both(f.y)));
+            s[x][nt][2 * half] = y.x;
+            s[x][nt][2 * half + 1] = y.y;
+          }
+      }
+    };
+    // One step: weights of the logits s, the running sums, the second product.
+    const int mat_row = ((lane >> 3) & 1) * 8 + (lane & 7);
+    const uint32_t v_lane = Sh::kValues + value_offset<D>(mat_row, lane >> 4);
+    auto step = [&](int i, int p0, float (&s)[kPass][NT][4]) {
+      const uint32_t stage = ring_u + (i % kAttnStages) * Sh::kStage;
+      const int tb = t0 + kAttnRun * (sub_warp + head_warps * i) + p0 * 16;
+      float2 unscale[NT];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) unscale[nt] = kRowScale ? lds_float2(qrow_u + nt * 64 + 8) : both(1.0f);
+      float2 vf[kPass][2];  // a token's value scale, and its minimum
+#pragma unroll
+      for (int x = 0; x < kPass; ++x)
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+          vf[x][half] = lds_float2(stage + Sh::kFactors + ((p0 + x) * 16 + half * 8 + g) * 16 + 8);
+      bool apart = false;
+      if (tb + kPass * 16 > min(lim_first, t1)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int lim = min(limit(nt * 8 + 2 * t + c), t1);
+#pragma unroll
+            for (int x = 0; x < kPass; ++x)
+#pragma unroll
+              for (int half = 0; half < 2; ++half)
+                if (tb + x * 16 + half * 8 + g >= lim) s[x][nt][2 * half + c] = -INFINITY;
+          }
+        // A hidden token's zero weight hides its value, unless that is a NaN or an infinity.
+        float odd = 0.0f;
+#pragma unroll
+        for (int x = 0; x < kPass; ++x)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) odd = fmaf(vf[x][half].x, 0.0f, fmaf(vf[x][half].y, 0.0f, odd));
+        apart = __any_sync(0xffffffffu, odd != 0.0f);
+      }
+
+      float2 l_new[NT], r_new[NT];
+      uint32_t wh[kPass][NT][2];
+      uint32_t top;  // the largest weights, a NaN before all (0 * infinity, of a logit far past the reference, is one)
+      auto weigh = [&](auto masked) {
+        top = 0;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          l_new[nt] = l[nt];
+          r_new[nt] = r[nt];
+#pragma unroll
+          for (int x = 0; x < kPass; ++x)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const float2 sv = make_float2(s[x][nt][2 * half], s[x][nt][2 * half + 1]);
+              const float2 dv = kRowScale ? fma2_f32(sv, unscale[nt], nref[nt]) : add2_f32(sv, nref[nt]);
+              const float2 p = make_float2(ex2(dv.x), ex2(dv.y));
+              float2 w = mul2_f32(p, mul2_f32(wscale[nt], both(vf[x][half].x)));
+              float2 vmh = both(vf[x][half].y);
+              if (masked.value) {
+                w.x = sv.x == -INFINITY ? 0.0f : w.x;
+                w.y = sv.y == -INFINITY ? 0.0f : w.y;
+                vmh.x = sv.x == -INFINITY ? 0.0f : vmh.x;
+                vmh.y = sv.y == -INFINITY ? 0.0f : vmh.y;
+              }
+              l_new[nt] = add2_f32(l_new[nt], p);
+              r_new[nt] = fma2_f32(p, vmh, r_new[nt]);
+              wh[x][nt][half] = Elem<__half>::from_f2(w.x, w.y);
+              top = max_nan_half2(top, wh[x][nt][half]);
+            }
+        }
+      };
+      weigh(std::false_type{});
+      if (apart) weigh(std::true_type{});
+      const bool first = i == 0 && p0 == 0;
+      // The references move only when a weight passes 1024 (fp32 sums and fp16 weights have that much room), and with
+      // the first step: the accumulators are then rescaled, which most steps need not do. A half above 1024
+      // (0x6400), an infinity or a NaN carries into its sign bit.
+      if (first || __any_sync(0xffffffffu, (top + 0x1bff1bffu) & 0x80008000u)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float hi[2] = {-INFINITY, -INFINITY}, hw[2] = {-INFINITY, -INFINITY}, seen[2] = {l[nt].x, l[nt].y};
+#pragma unroll
+          for (int x = 0; x < kPass; ++x)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const float lv = __log2f(vf[x][half].x);
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                const float logit = s[x][nt][2 * half + c] * (c == 0 ? unscale[nt].x : unscale[nt].y);
+                hi[c] = fmaxf(hi[c], logit);
+                hw[c] = fmaxf(hw[c], logit + lv);  // fmaxf passes over a NaN
+              }
+            }
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int z = 4; z < 32; z <<= 1) {
+              hi[c] = fmaxf(hi[c], __shfl_xor_sync(0xffffffffu, hi[c], z));
+              hw[c] = fmaxf(hw[c], __shfl_xor_sync(0xffffffffu, hw[c], z));
+              seen[c] = fmaxf(seen[c], __shfl_xor_sync(0xffffffffu, seen[c], z));
+            }
+          float fl[2], fo[2], nr[2] = {nref[nt].x, nref[nt].y}, ws[2] = {wscale[nt].x, wscale[nt].y};
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            // Only rows that need it move, so that no row's rounding depends on another's values. Then the largest
+            // weight of the row so far (at most 1024 by the scale it has) or of this step becomes at most 1.
+            const float old = seen[c] == 0.0f ? -INFINITY : -nr[c];
+            const float was = old - __log2f(ws[c]);
+            fl[c] = fo[c] = 1.0f;
+            if (!(hw[c] > was + 10.0f || hi[c] > old + 100.0f)) continue;
+            const float now = fmaxf(old, hi[c]);
+            const float room = floorf(now - fmaxf(was, hw[c]));
+            const float nws = now == -INFINITY ? 1.0f : __uint_as_float((uint32_t)(fminf(fmaxf(room, -126.0f), 127.0f) + 127.0f) << 23);
+            fl[c] = now == old ? 1.0f : ex2(old - now);
+            fo[c] = fl[c] * (nws / ws[c]);
+            nr[c] = now == -INFINITY ? 0.0f : -now;
+            ws[c] = nws;
+          }
+          nref[nt] = make_float2(nr[0], nr[1]);
+          wscale[nt] = make_float2(ws[0], ws[1]);
+          l[nt].x *= fl[0]; l[nt].y *= fl[1];
+          r[nt].x *= fl[0]; r[nt].y *= fl[1];
+#pragma unroll
+          for (int j = 0; j < kMt; ++j) {
+            o[j][nt][0] *= fo[0]; o[j][nt][1] *= fo[1];
+            o[j][nt][2] *= fo[0]; o[j][nt][3] *= fo[1];
+          }
+          if (kCentred) {
+            wsum[nt][0] *= fo[0]; wsum[nt][1] *= fo[1];
+            wsum[nt][2] *= fo[0]; wsum[nt][3] *= fo[1];
+          }
+        }
+        if (apart) weigh(std::true_type{}); else weigh(std::false_type{});
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        l[nt] = l_new[nt];
+        r[nt] = r_new[nt];
+      }
+#pragma unroll
+      for (int x = 0; x < kPass; ++x)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) wh[x][nt][half] = transpose8x8(wh[x][nt][half]);
+      if (kCentred) {
+        constexpr uint32_t kOnes = 0x3c003c00u;
+#pragma unroll
+        for (int x = 0; x < kPass; ++x)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            mma_fp16(wsum[nt], kOnes, kOnes, kOnes, kOnes, wh[x][nt][0], wh[x][nt][1]);
+      }
+
+      // The second product, D x rows over 16 tokens: a unit of four codes of tokens 2t, 2t + 1 (ab) and 2t + 8, 2t + 9 (cd)
+      // comes transposed from shared memory, 32 elements of D a chunk.
+#pragma unroll
+      for (int x = 0; x < kPass; ++x)
+#pragma unroll
+        for (int c = 0; c < D / 32; c += 2) {
+          uint32_t u[4];
+          load_transposed(u, (stage + v_lane + (p0 + x) * 16 * Sh::kRowBytes) ^ (c * 16));
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            uint32_t ab[4], cd[4];
+            nibbles_fp16(u[2 * k], ab);
+            nibbles_fp16(u[2 * k + 1], cd);
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+                mma_fp16(o[2 * (c + k) + e][nt], ab[2 * e], ab[2 * e + 1], cd[2 * e], cd[2 * e + 1], wh[x][nt][0], wh[x][nt][1]);
+          }
+        }
+    };
 
     for (int i = 0; i < runs; ++i) {
       cp_async_wait<kAttnStages - 2>();
@@ -412,249 +706,129 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtasPerSm) attn_int4_kernel
         issue(i + kAttnStages - 1, page);
         page = next;
       }
-      const uint32_t stage = ring_u + (i % kAttnStages) * Sh::kStage;
-      const int tb = t0 + kAttnRun * (warp + kAttnWarps * i);
-
-      float s[4][4];
-      uint32_t kw[4][kWords];
+      make_factors(i);
 #pragma unroll
-      for (int nt = 0; nt < 4; ++nt) {
-        const uint32_t at_row = stage + Sh::kKeys + (nt * 8 + g) * Sh::kRowBytes + t * (D / 8);
-        if (D == 128) {
-          const uint4 v = lds128(at_row);
-          kw[nt][0] = v.x; kw[nt][1] = v.y; kw[nt][kWords - 2] = v.z; kw[nt][kWords - 1] = v.w;
-        } else {
-          const uint2 v = lds64(at_row);
-          kw[nt][0] = v.x; kw[nt][1] = v.y;
-        }
-        s[nt][0] = s[nt][1] = Keys::kStart * qsum0;
-        s[nt][2] = s[nt][3] = Keys::kStart * qsum1;
-      }
-#pragma unroll
-      for (int w = 0; w < kWords; ++w) {
-        const uint4 qa = lds128(qfrag_u + (2 * w * 32 + lane) * 16);
-        const uint4 qb = lds128(qfrag_u + ((2 * w + 1) * 32 + lane) * 16);
-#pragma unroll
-        for (int nt = 0; nt < 4; ++nt) {
-          uint32_t p[4];
-          Keys::unpack(kw[nt][w], p);
-          Keys::mma(s[nt], qa, p[0], p[1]);
-          Keys::mma(s[nt], qb, p[2], p[3]);
-        }
-      }
-
-      // The pairs: logits in units of log2, and what the values need of each token.
-      float vs[4][2], vm[4][2];
-#pragma unroll
-      for (int nt = 0; nt < 4; ++nt) {
-        const uint4 v = lds128(stage + Sh::kPairs + nt * 64 + t * 16);
-        const uint32_t kp[2] = {v.x, v.z}, vp[2] = {v.y, v.w};
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const float sk = __uint_as_float(kp[c] << 16);
-          const float km = __uint_as_float(kp[c] & 0xffff0000u);
-          const float ks = sk * a.scale_log2, kb = fmaf(Keys::kCentre, sk, km) * a.scale_log2;
-          vs[nt][c] = __uint_as_float(vp[c] << 16);
-          vm[nt][c] = fmaf(8.0f, vs[nt][c], __uint_as_float(vp[c] & 0xffff0000u));
-          s[nt][c] = fmaf(s[nt][c], ks, qsum0 * kb);
-          s[nt][2 + c] = fmaf(s[nt][2 + c], ks, qsum1 * kb);
-        }
-      }
-      const bool edge = tb + kAttnRun > min(lim_first, t1);
-      if (edge) {
-#pragma unroll
-        for (int nt = 0; nt < 4; ++nt)
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const int tok = tb + nt * 8 + 2 * t + c;
-            if (tok >= lim0 || tok >= t1) s[nt][c] = -INFINITY;
-            if (tok >= lim1 || tok >= t1) s[nt][2 + c] = -INFINITY;
-          }
-      }
-      float x0 = -INFINITY, x1 = -INFINITY;
-#pragma unroll
-      for (int nt = 0; nt < 4; ++nt) {
-        x0 = fmaxf(x0, fmaxf(s[nt][0], s[nt][1]));
-        x1 = fmaxf(x1, fmaxf(s[nt][2], s[nt][3]));
-      }
-      x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 1));
-      x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2));
-      x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
-      x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2));
-      // The reference point of the exponentials moves only when a logit passes it by 8 (a factor of 256,
-      // harmless in fp32 and bf16): the accumulators are then rescaled, which most runs need not do.
-      if (__any_sync(0xffffffffu, x0 > m0 + 8.0f || x1 > m1 + 8.0f)) {
-        const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
-        const float f0 = n0 == m0 ? 1.0f : ex2(m0 - n0), f1 = n1 == m1 ? 1.0f : ex2(m1 - n1);
-        m0 = n0;
-        m1 = n1;
-        l0 *= f0; r0 *= f0;
-        l1 *= f1; r1 *= f1;
-#pragma unroll
-        for (int j = 0; j < kNt; ++j) {
-          o[j][0] *= f0; o[j][1] *= f0;
-          o[j][2] *= f1; o[j][3] *= f1;
-        }
-      }
-      const float ref0 = m0 == -INFINITY ? 0.0f : m0, ref1 = m1 == -INFINITY ? 0.0f : m1;
-      // A hidden token's terms are left out, not multiplied by its zero weight: its pair may be NaN.
-      auto weigh = [&](auto masked) {
-#pragma unroll
-        for (int nt = 0; nt < 4; ++nt)
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const bool in0 = !masked.value || s[nt][c] != -INFINITY, in1 = !masked.value || s[nt][2 + c] != -INFINITY;
-            const float p0 = ex2(s[nt][c] - ref0), p1 = ex2(s[nt][2 + c] - ref1);
-            l0 += p0;
-            l1 += p1;
-            r0 = in0 ? fmaf(p0, vm[nt][c], r0) : r0;
-            r1 = in1 ? fmaf(p1, vm[nt][c], r1) : r1;
-            s[nt][c] = in0 ? p0 * vs[nt][c] : 0.0f;
-            s[nt][2 + c] = in1 ? p1 * vs[nt][c] : 0.0f;
-          }
-      };
-      if (edge) weigh(std::true_type{}); else weigh(std::false_type{});
-
-#pragma unroll
-      for (int kk = 0; kk < 2; ++kk) {
-        float (&sa)[4] = s[2 * kk];
-        float (&sb)[4] = s[2 * kk + 1];
-        const uint4 hi = make_uint4(pack_bf16(sa[0], sa[1]), pack_bf16(sa[2], sa[3]), pack_bf16(sb[0], sb[1]),
-                                    pack_bf16(sb[2], sb[3]));
-        uint4 lo = make_uint4(0, 0, 0, 0);
-        if (sizeof(T) == 2 && Keys::kCentre != 0.0f) {  // fp16 queries: the rest of p sv
-          const float2 h0 = Elem<__nv_bfloat16>::to_f2(hi.x), h1 = Elem<__nv_bfloat16>::to_f2(hi.y);
-          const float2 h2 = Elem<__nv_bfloat16>::to_f2(hi.z), h3 = Elem<__nv_bfloat16>::to_f2(hi.w);
-          lo = make_uint4(pack_bf16(sa[0] - h0.x, sa[1] - h0.y), pack_bf16(sa[2] - h1.x, sa[3] - h1.y),
-                          pack_bf16(sb[0] - h2.x, sb[1] - h2.y), pack_bf16(sb[2] - h3.x, sb[3] - h3.y));
-        }
-        constexpr int kVWords = D / 64;
-        uint32_t vw[4][kVWords];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int row = 16 * kk + 2 * t + (x & 1) + 8 * (x >> 1);
-          const uint32_t src = stage + Sh::kValues + value_offset<D>(row, (g * (D / 16)) & ~15) + ((g * (D / 16)) & 15);
-          if (D == 128) {
-            const uint2 v = lds64(src);
-            vw[x][0] = v.x;
-            vw[x][kVWords - 1] = v.y;
-          } else {
-            vw[x][0] = lds32(src);
-          }
-        }
-#pragma unroll
-        for (int w = 0; w < kVWords; ++w) {
-          const uint32_t ab[2] = {__byte_perm(vw[0][w], vw[1][w], 0x5410), __byte_perm(vw[0][w], vw[1][w], 0x7632)};
-          const uint32_t cd[2] = {__byte_perm(vw[2][w], vw[3][w], 0x5410), __byte_perm(vw[2][w], vw[3][w], 0x7632)};
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const uint32_t b0 = value_codes(ab[e >> 2], e & 3), b1 = value_codes(cd[e >> 2], e & 3);
-            mma_bf16(o[8 * w + e], hi.x, hi.y, hi.z, hi.w, b0, b1);
-            if (sizeof(T) == 2 && Keys::kCentre != 0.0f) mma_bf16(o[8 * w + e], lo.x, lo.y, lo.z, lo.w, b0, b1);
-          }
-        }
+      for (int p0 = 0; p0 < 2; p0 += kPass) {
+        float s[kPass][NT][4];
+        logits(i, p0, s);
+        step(i, p0, s);
       }
     }
     cp_async_wait<0>();
 
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-    r0 += __shfl_xor_sync(0xffffffffu, r0, 1);
-    r0 += __shfl_xor_sync(0xffffffffu, r0, 2);
-    r1 += __shfl_xor_sync(0xffffffffu, r1, 1);
-    r1 += __shfl_xor_sync(0xffffffffu, r1, 2);
+    // A row's sums over the lanes that hold its other tokens.
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int z = 4; z < 32; z <<= 1) {
+        l[nt].x += __shfl_xor_sync(0xffffffffu, l[nt].x, z);
+        l[nt].y += __shfl_xor_sync(0xffffffffu, l[nt].y, z);
+        r[nt].x += __shfl_xor_sync(0xffffffffu, r[nt].x, z);
+        r[nt].y += __shfl_xor_sync(0xffffffffu, r[nt].y, z);
+      }
 
-    // Join the warps: statistics, then o (with the minima's part added), lane by lane.
-    if (t == 0) {
-      stats[(warp * kAttnRows + g) * 2] = m0;
-      stats[(warp * kAttnRows + g) * 2 + 1] = l0;
-      stats[(warp * kAttnRows + g + 8) * 2] = m1;
-      stats[(warp * kAttnRows + g + 8) * 2 + 1] = l1;
+    // Join a head's warps, o and r of each relative to its own reference m.
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      if (g == 0) {
+        float* st = stats + (warp * kRows + nt * 8 + 2 * t) * 2;
+        st[0] = l[nt].x == 0.0f ? -INFINITY : -nref[nt].x; st[1] = l[nt].x;
+        st[2] = l[nt].y == 0.0f ? -INFINITY : -nref[nt].y; st[3] = l[nt].y;
+      }
     }
     __syncthreads();  // all rings are drained: their memory may be overwritten
 #pragma unroll
-    for (int j = 0; j < kNt; ++j) {
-      merge[((warp * kNt + j) * 4 + 0) * 32 + lane] = o[j][0] + r0;
-      merge[((warp * kNt + j) * 4 + 1) * 32 + lane] = o[j][1] + r0;
-      merge[((warp * kNt + j) * 4 + 2) * 32 + lane] = o[j][2] + r1;
-      merge[((warp * kNt + j) * 4 + 3) * 32 + lane] = o[j][3] + r1;
+    for (int nt = 0; nt < NT; ++nt) {
+      const float b0 = 1.0f / wscale[nt].x, b1 = 1.0f / wscale[nt].y;
+      const float w0 = kCentred ? kCentre * wsum[nt][0] : 0.0f, w1 = kCentred ? kCentre * wsum[nt][1] : 0.0f;
+#pragma unroll
+      for (int j = 0; j < kMt; ++j) {
+        float* dst = merge + ((warp * kMt + j) * NT + nt) * 128 + lane;
+        dst[0] = fmaf(fmaf(o[j][nt][0], kEvenUnit, -w0), b0, r[nt].x);
+        dst[32] = fmaf(fmaf(o[j][nt][1], kEvenUnit, -w1), b1, r[nt].y);
+        dst[64] = fmaf(fmaf(o[j][nt][2], kOddUnit, -w0), b0, r[nt].x);
+        dst[96] = fmaf(fmaf(o[j][nt][3], kOddUnit, -w1), b1, r[nt].y);
+      }
     }
     __syncthreads();
     const bool starts = unit == 0, ends = unit + seg_units == rq.units;
     const int slot = starts && !ends ? 1 : 0;
-    float* part = a.part + ((int64_t)blockIdx.x * 2 + slot) * attn_part_floats(D);
+    float* part = a.part + (((int64_t)blockIdx.x * 2 + slot) * cta_heads + which) * attn_part_floats(D, NT);
+    const int first_warp = which * head_warps;
+    // This warp's share of the D tiles.
+    const int tiles_here = kMt / head_warps;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int r = g + 8 * half;
-      float top = -INFINITY, sum = 0.0f, f[kAttnWarps];
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int w = 0; w < kAttnWarps; ++w) top = fmaxf(top, stats[(w * kAttnRows + r) * 2]);
+      for (int c = 0; c < 2; ++c) {
+        const int rr = nt * 8 + 2 * t + c;
+        float top = -INFINITY, sum = 0.0f, f[kAttnWarps];
 #pragma unroll
-      for (int w = 0; w < kAttnWarps; ++w) {
-        const float mw = stats[(w * kAttnRows + r) * 2];
-        f[w] = mw == top ? 1.0f : ex2(mw - top);
-        sum = fmaf(f[w], stats[(w * kAttnRows + r) * 2 + 1], sum);
-      }
-      if (r < rows_here) {
-        const int tok = (row0 + r) / a.group, sub = (row0 + r) - tok * a.group;
-        const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;  // a row that sees no key is zero
-        // This warp's quarter of the columns: kNt / 4 consecutive elements of each of the lane's two stretches.
+        for (int w = 0; w < kAttnWarps; ++w)
+          if (w < head_warps) top = fmaxf(top, stats[((first_warp + w) * kRows + rr) * 2]);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          float v[kNt / 4];
-#pragma unroll
-          for (int jj = 0; jj < kNt / 4; ++jj) {
-            const int j = warp * (kNt / 4) + jj;
-            float x = 0.0f;
+        for (int w = 0; w < kAttnWarps; ++w) {
+          f[w] = 0.0f;
+          if (w < head_warps) {
+            const float mw = stats[((first_warp + w) * kRows + rr) * 2];
+            f[w] = mw == top ? 1.0f : ex2(mw - top);
+            sum = fmaf(f[w], stats[((first_warp + w) * kRows + rr) * 2 + 1], sum);
+          }
+        }
+        if (rr < rows_here) {
+          const int tok = (row0 + rr) / a.group, sub = (row0 + rr) - tok * a.group;
+          const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;  // a row that sees no key is zero
+          uint16_t* dst = static_cast<uint16_t*>(a.out) + (int64_t)(rq.q0 + tok) * a.osn +
+                          ((int64_t)head * a.group + sub) * a.osh;
+          for (int jj = 0; jj < tiles_here; ++jj) {
+            const int j = sub_warp * tiles_here + jj;
+            float v0 = 0.0f, v1 = 0.0f;
 #pragma unroll
             for (int w = 0; w < kAttnWarps; ++w)
-              x = fmaf(f[w], merge[((w * kNt + j) * 4 + 2 * half + c) * 32 + lane], x);
-            v[jj] = x;
+              if (w < head_warps) {
+                const float* src = merge + (((first_warp + w) * kMt + j) * NT + nt) * 128 + c * 32 + lane;
+                v0 = fmaf(f[w], src[0], v0);
+                v1 = fmaf(f[w], src[64], v1);
+              }
+            const int d = 32 * (j >> 1) + 4 * g + 2 * (j & 1);
+            if (starts && ends) {
+              dst[d] = Elem<T>::from_f(v0 * inv);
+              dst[d + 1] = Elem<T>::from_f(v1 * inv);
+            } else {
+              *reinterpret_cast<float2*>(part + rr * D + d) = make_float2(v0, v1);
+            }
           }
-          const int d0 = (D / 8) * (2 * t + c) + warp * (kNt / 4);
-          if (starts && ends) {
-            uint16_t* dst = static_cast<uint16_t*>(a.out) + (int64_t)(rq.q0 + tok) * a.osn +
-                            ((int64_t)head * a.group + sub) * a.osh + d0;
-#pragma unroll
-            for (int jj = 0; jj < kNt / 4; ++jj) dst[jj] = Elem<T>::from_f(v[jj] * inv);
-          } else {
-#pragma unroll
-            for (int jj = 0; jj < kNt / 4; ++jj) part[r * D + d0 + jj] = v[jj];
-          }
-        }
-        if (warp == 0 && t == 0) {
-          if (starts && ends) {
-            if (a.lse != nullptr)
-              a.lse[(int64_t)(rq.q0 + tok) * heads * a.group + (int64_t)head * a.group + sub] =
-                  sum != 0.0f ? top + __log2f(sum) : -INFINITY;
-          } else {
-            part[kAttnRows * D + 2 * r] = top;
-            part[kAttnRows * D + 2 * r + 1] = sum;
+          if (sub_warp == 0 && g == 0) {
+            if (starts && ends) {
+              if (a.lse != nullptr)
+                a.lse[(int64_t)(rq.q0 + tok) * a.kv.heads * a.group + (int64_t)head * a.group + sub] =
+                    sum != 0.0f ? top + __log2f(sum) : -INFINITY;
+            } else {
+              part[kRows * D + 2 * rr] = top;
+              part[kRows * D + 2 * rr + 1] = sum;
+            }
           }
         }
       }
-    }
     if (starts && !ends) {
       // The tile goes on in the following CTAs, up to the one that holds its last unit.
       const int64_t last = (at + rq.units - 1) / share;
       desc_parts = (int)(last - blockIdx.x) + 1;
       desc_request = b;
-      desc_row = tile * kAttnRows;
-      desc_head = head;
+      desc_row = row0;
+      desc_head = head_group * cta_heads;
     }
     __syncthreads();  // merge and the queries may be overwritten
 
     at += seg_units;
     unit += seg_units;
     if (unit == rq.units && at < end) {
-      unit = 0;
-      if (++head == heads) {
-        head = 0;
+      unit = -kAttnLead;
+      if (++head_group == head_groups) {
+        head_group = 0;
         if (++tile == rq.tiles) {
           tile = 0;
-          do rq = attn_request(a, ++b, nullptr); while (rq.tiles == 0);  // at < end: there is one
+          do rq = attn_request<kRows>(a, ++b, nullptr); while (rq.tiles == 0);  // at < end: there is one
         }
       }
     }
@@ -668,27 +842,29 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtasPerSm) attn_int4_kernel
   pdl_launch_dependents();
 }
 
-// Joins the parts of the tiles that were split: CTA (c, y) takes rows 4y .. 4y + 3 of the tile that the
-// main kernel's CTA c started, a warp a row, in the order of the parts.
-template <typename T, int D>
+// Joins the parts of the tiles that were split: CTA (c, y) takes four (head, row) pairs of the tile that the
+// main kernel's CTA c started, a warp each, in the order of the parts.
+template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kAttnThreads) attn_int4_join_kernel(const AttnInt4Args a) {
+  constexpr int kRows = 8 * NT;
   pdl_wait();
   const int lane = threadIdx.x & 31;
-  const int r = blockIdx.y * kAttnWarps + (threadIdx.x >> 5);
+  const int hr = blockIdx.y * kAttnWarps + (threadIdx.x >> 5);
+  const int which = hr / kRows, r = hr % kRows;
   const int32_t* desc = a.desc + (int64_t)blockIdx.x * kAttnDescInts;
   const int parts = desc[0];
   if (parts > 0) {
-    const AttnRequest rq = attn_request(a, desc[1], nullptr);
-    const int row = desc[2] + r, head = desc[3];
+    const AttnRequest rq = attn_request<kRows>(a, desc[1], nullptr);
+    const int row = desc[2] + r, head = desc[3] + which;
     if (row < rq.qlen * a.group) {
       constexpr int kPer = D / 32;
-      const int64_t stride = 2 * attn_part_floats(D);
+      const int64_t slot = (int64_t)a.cta_heads * attn_part_floats(D, NT);
       // part 0 is slot 1 of CTA c, part i slot 0 of CTA c + i
-      const float* first = a.part + ((int64_t)blockIdx.x * 2 + 1) * attn_part_floats(D);
-      const float* rest = a.part + (int64_t)blockIdx.x * stride;
+      const float* rest = a.part + blockIdx.x * 2 * slot + which * attn_part_floats(D, NT);
+      const float* first = rest + slot;
       float top = -INFINITY;
       for (int i = lane; i < parts; i += 32)
-        top = fmaxf(top, (i == 0 ? first : rest + i * stride)[kAttnRows * D + 2 * r]);
+        top = fmaxf(top, (i == 0 ? first : rest + i * 2 * slot)[kRows * D + 2 * r]);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
       float sum = 0.0f, acc[kPer];
@@ -696,8 +872,8 @@ __global__ void __launch_bounds__(kAttnThreads) attn_int4_join_kernel(const Attn
       for (int j = 0; j < kPer; ++j) acc[j] = 0.0f;
 #pragma unroll 4
       for (int i = 0; i < parts; ++i) {
-        const float* p = i == 0 ? first : rest + i * stride;
-        const float m = p[kAttnRows * D + 2 * r], l = p[kAttnRows * D + 2 * r + 1];
+        const float* p = i == 0 ? first : rest + i * 2 * slot;
+        const float m = p[kRows * D + 2 * r], l = p[kRows * D + 2 * r + 1];
         const float f = m == top ? 1.0f : ex2(m - top);
         sum = fmaf(f, l, sum);
 #pragma unroll

@@ -112,6 +112,17 @@ cudaError_t opt_in_rope_ring() {
   return opt_in_smem(rope_ring_kernel<T, int64_t, false, true>);
 }
 
+template <typename T>
+cudaError_t opt_in_attn_int4() {
+  cudaError_t e;
+  if ((e = opt_in_smem(attn_int4_kernel<T, 64, 1>, AttnInt4Shape<64, 1>::kSmem)) != cudaSuccess) return e;
+  if ((e = opt_in_smem(attn_int4_kernel<T, 64, 2>, AttnInt4Shape<64, 2>::kSmem)) != cudaSuccess) return e;
+  if ((e = opt_in_smem(attn_int4_kernel<T, 64, 4>, AttnInt4Shape<64, 4>::kSmem)) != cudaSuccess) return e;
+  if ((e = opt_in_smem(attn_int4_kernel<T, 128, 1>, AttnInt4Shape<128, 1>::kSmem)) != cudaSuccess) return e;
+  if ((e = opt_in_smem(attn_int4_kernel<T, 128, 2>, AttnInt4Shape<128, 2>::kSmem)) != cudaSuccess) return e;
+  return opt_in_smem(attn_int4_kernel<T, 128, 4>, AttnInt4Shape<128, 4>::kSmem);
+}
+
 cudaError_t prepare_current(DeviceState& st, int device) {
   cudaError_t e = cudaDeviceGetAttribute(&st.sm_count, cudaDevAttrMultiProcessorCount, device);
   if (e != cudaSuccess) return e;
@@ -134,10 +145,8 @@ cudaError_t prepare_current(DeviceState& st, int device) {
   if ((e = opt_in_smem(paged_alloc_kernel<false, true>, kAllocSmemMax)) != cudaSuccess) return e;
   if ((e = opt_in_smem(paged_alloc_kernel<true, false>, kAllocSmemMax)) != cudaSuccess) return e;
   if ((e = opt_in_smem(paged_alloc_kernel<true, true>, kAllocSmemMax)) != cudaSuccess) return e;
-  if ((e = opt_in_smem(attn_int4_kernel<__nv_bfloat16, 64>, AttnInt4Shape<64>::kSmem)) != cudaSuccess) return e;
-  if ((e = opt_in_smem(attn_int4_kernel<__nv_bfloat16, 128>, AttnInt4Shape<128>::kSmem)) != cudaSuccess) return e;
-  if ((e = opt_in_smem(attn_int4_kernel<__half, 64>, AttnInt4Shape<64>::kSmem)) != cudaSuccess) return e;
-  if ((e = opt_in_smem(attn_int4_kernel<__half, 128>, AttnInt4Shape<128>::kSmem)) != cudaSuccess) return e;
+  if ((e = opt_in_attn_int4<__nv_bfloat16>()) != cudaSuccess) return e;
+  if ((e = opt_in_attn_int4<__half>()) != cudaSuccess) return e;
   void* fault = nullptr;
   if ((e = cudaGetSymbolAddress(&fault, g_fault_word)) != cudaSuccess) return e;
   st.fault = static_cast<int32_t*>(fault);
@@ -688,29 +697,47 @@ int run_kv_int4(KVInt4RowArgs a, const MasInt4KVCache* cache, int64_t num_kv_hea
              : launch_kv_int4_t<READ, T, int32_t, 64>(a, vec, st, stream, enable_pdl);
 }
 
-// The workspace of an attention launch: every CTA's two parts, then its descriptor.
-int64_t attn_ctas(const DeviceState& st) { return (int64_t)st.sm_count * kAttnCtasPerSm; }
+// The workspace of an attention launch: every CTA's two parts, then its descriptor; sized for the tile height
+// that needs most.
+int64_t attn_ctas(const DeviceState& st, int NT) {
+  return (int64_t)st.sm_count * (NT == 1 ? AttnInt4Shape<128, 1>::kCtasPerSm
+                                         : NT == 2 ? AttnInt4Shape<128, 2>::kCtasPerSm : AttnInt4Shape<128, 4>::kCtasPerSm);
+}
 int64_t attn_part_bytes(const DeviceState& st, int64_t head_size) {
-  return attn_ctas(st) * 2 * attn_part_floats((int)head_size) * (int64_t)sizeof(float);
+  int64_t most = 0;
+  for (int nt = 1; nt <= 4; nt *= 2)
+    most = std::max(most, attn_ctas(st, nt) * 2 * kAttnMaxHeads * attn_part_floats((int)head_size, nt));
+  return most * (int64_t)sizeof(float);
 }
 int64_t attn_workspace_bytes(const DeviceState& st, int64_t head_size) {
-  return attn_part_bytes(st, head_size) + attn_ctas(st) * kAttnDescInts * (int64_t)sizeof(int32_t);
+  return attn_part_bytes(st, head_size) + std::max({attn_ctas(st, 1), attn_ctas(st, 2), attn_ctas(st, 4)}) * kAttnDescInts * (int64_t)sizeof(int32_t);
+}
+
+template <typename T, int D, int NT>
+int launch_attn_int4(AttnInt4Args a, DeviceState* st, void* stream, int enable_pdl) {
+  // Upper bounds on the units of work: the lengths are known to the device only.
+  const int64_t ctas = attn_ctas(*st, NT);
+  const int64_t unit = kAttnRun * (kAttnWarps / a.cta_heads);
+  const int64_t tiles = ceil_div(a.T * a.group, 8 * NT) + a.B;
+  const int64_t max_units = std::max<int64_t>(1, ceil_div((int64_t)a.max_blocks * a.kv.page_size, unit));
+  const int64_t bound = std::min(tiles * (a.kv.heads / a.cta_heads), ctas) * std::min(max_units, ctas);
+  const unsigned grid = (unsigned)std::min(bound, ctas);
+  const bool split = max_units > 1;
+  if (!split) a.desc = nullptr;
+  const int rc = launch(attn_int4_kernel<T, D, NT>, dim3(grid), dim3(kAttnThreads), AttnInt4Shape<D, NT>::kSmem, stream,
+                        enable_pdl, a);
+  if (rc != MAS_OK || !split) return rc;
+  return launch(attn_int4_join_kernel<T, D, NT>, dim3(grid, a.cta_heads * 8 * NT / kAttnWarps), dim3(kAttnThreads), 0,
+                stream, enable_pdl, a);
 }
 
 template <typename T, int D>
-int launch_attn_int4(AttnInt4Args a, DeviceState* st, void* stream, int enable_pdl) {
-  // Upper bounds on the units of work: the lengths are known to the device only.
-  const int64_t tiles = ceil_div(a.T * a.group, kAttnRows) + a.B;
-  const int64_t max_units = std::max<int64_t>(1, ceil_div((int64_t)a.max_blocks * a.kv.page_size, kAttnUnit));
-  const int64_t bound = std::min(tiles * a.kv.heads, attn_ctas(*st)) * std::min(max_units, attn_ctas(*st));
-  const unsigned grid = (unsigned)std::min(bound, attn_ctas(*st));
-  const bool split = max_units > 1;
-  if (!split) a.desc = nullptr;
-  const int rc = launch(attn_int4_kernel<T, D>, dim3(grid), dim3(kAttnThreads), AttnInt4Shape<D>::kSmem, stream,
-                        enable_pdl, a);
-  if (rc != MAS_OK || !split) return rc;
-  return launch(attn_int4_join_kernel<T, D>, dim3(grid, kAttnRows / kAttnWarps), dim3(kAttnThreads), 0, stream,
-                enable_pdl, a);
+int run_attn_int4(const AttnInt4Args& a, DeviceState* st, void* stream, int enable_pdl) {
+  // Rows that share a request's kv head, on average: the tile takes them in one go up to 32.
+  const int64_t rows = ceil_div(a.T, a.B) * a.group;
+  if (rows <= 8) return launch_attn_int4<T, D, 1>(a, st, stream, enable_pdl);
+  if (rows <= 16) return launch_attn_int4<T, D, 2>(a, st, stream, enable_pdl);
+  return launch_attn_int4<T, D, 4>(a, st, stream, enable_pdl);
 }
 
 }  // namespace
@@ -1280,6 +1307,10 @@ int mas_paged_attention_int4(const void* query, void* out, float* lse, const Mas
       out_stride_head < 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads != 0 ||
       (cum_seq_lens_q == nullptr && num_tokens != batch_size))
     return MAS_ERR_INVALID_ARGUMENT;
+  // The kernel's offsets into the codes are 32 bits of 16 bytes.
+  const int64_t last = (a.kv.num_pages - 1) * (a.kv.stride_page >> 4) + (a.kv.page_size - 1) * (a.kv.stride_entry >> 4) +
+                       (num_kv_heads - 1) * (a.kv.stride_head >> 4) + head_size / 32;
+  if (a.kv.num_pages > 0 && last > (int64_t)UINT32_MAX) return MAS_ERR_UNSUPPORTED_SHAPE;
   if (num_q_heads > INT32_MAX || num_tokens > INT32_MAX / num_q_heads) return MAS_ERR_UNSUPPORTED_SHAPE;
   if (batch_size == 0 || num_tokens == 0) return MAS_OK;
   if (!query || !out || !seq_lens || (max_blocks > 0 && !block_tables)) return MAS_ERR_INVALID_ARGUMENT;
@@ -1298,13 +1329,17 @@ int mas_paged_attention_int4(const void* query, void* out, float* lse, const Mas
   if ((a.kv.page_size & (a.kv.page_size - 1)) == 0)
     for (a.page_shift = 0; (1ll << a.page_shift) < a.kv.page_size; ++a.page_shift) {}
   a.causal = causal ? 1 : 0;
+  a.cta_heads = num_kv_heads % 2 == 0 ? 2 : 1;
+  a.q_vec = aligned(query, 16) && q_stride_token % 8 == 0 && q_stride_head % 8 == 0;
+  a.page16 = (uint32_t)(a.kv.stride_page >> 4);
+  a.entry16 = (uint32_t)(a.kv.stride_entry >> 4);
   a.status = status != nullptr ? status : st->status;
   const bool big = head_size == 128;
   if (dtype == MAS_DTYPE_BF16)
-    return big ? launch_attn_int4<__nv_bfloat16, 128>(a, st, stream, enable_pdl)
-               : launch_attn_int4<__nv_bfloat16, 64>(a, st, stream, enable_pdl);
-  return big ? launch_attn_int4<__half, 128>(a, st, stream, enable_pdl)
-             : launch_attn_int4<__half, 64>(a, st, stream, enable_pdl);
+    return big ? run_attn_int4<__nv_bfloat16, 128>(a, st, stream, enable_pdl)
+               : run_attn_int4<__nv_bfloat16, 64>(a, st, stream, enable_pdl);
+  return big ? run_attn_int4<__half, 128>(a, st, stream, enable_pdl)
+             : run_attn_int4<__half, 64>(a, st, stream, enable_pdl);
 }
 
 }  // extern "C"
