@@ -12,6 +12,11 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
 
+#include <cmath>
+#include <optional>
+#include <string>
+#include <tuple>
+
 #include "../../include/mas_b200.h"
 
 namespace {
@@ -28,8 +33,10 @@ int id_code(const at::Tensor& t) {
   TORCH_CHECK(false, "mas_b200: indices must be int32 or int64, got ", t.scalar_type());
 }
 
+// Numbers go into messages as std::to_string: streaming an integer from this library crashed on a machine whose process
+// had a second C++ runtime's locale facets loaded.
 void check(int rc, const char* fn) {
-  TORCH_CHECK(rc == MAS_OK, fn, " failed with status ", rc, ": ", mas_status_string(rc));
+  TORCH_CHECK(rc == MAS_OK, fn, " failed with status ", std::to_string(rc), ": ", mas_status_string(rc));
 }
 
 // [rows, cols] view of a tensor whose last dimension is contiguous and whose leading dimensions
@@ -268,10 +275,28 @@ void embedding_out(at::Tensor out, at::Tensor input_ids, at::Tensor weight, bool
 }
 
 // ------------------------------------------------------------------------------------------------
-// The 4-bit paged cache.
+// The 4-bit paged cache. These operators check their arguments here (ValueError, as the Python layer's checks
+// elsewhere) and allocate what they return: a decode step calls several of them a layer, and a dozen attribute
+// reads and allocations from Python cost more than the kernels of a small step.
 // ------------------------------------------------------------------------------------------------
-void check_int32(const at::Tensor& t, const char* name) {
-  TORCH_CHECK(t.scalar_type() == at::kInt && t.is_contiguous(), "mas_b200: ", name, " must be contiguous int32");
+void same_device(const at::Tensor& ref, std::initializer_list<const at::Tensor*> others) {
+  for (const at::Tensor* t : others)
+    TORCH_CHECK(t->device() == ref.device(), "Expected all tensors to be on the same device, but found ", t->device(),
+                " beside ", ref.device());
+}
+
+void check_int32(const at::Tensor& t, const char* name, int64_t entries = -1) {
+  TORCH_CHECK_VALUE(t.scalar_type() == at::kInt && t.is_contiguous() && t.dim() == 1,
+                    name, " must be a contiguous int32 vector");
+  TORCH_CHECK_VALUE(entries < 0 || t.numel() == entries, name, " must have ", std::to_string(entries), " entries, got ",
+                    std::to_string(t.numel()));
+}
+
+// Index vectors of either integer type, as the kernels read them.
+at::Tensor as_int32(const at::Tensor& t, const char* name) {
+  if (t.scalar_type() == at::kInt && t.is_contiguous()) return t;
+  TORCH_CHECK_VALUE(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, name, " must be int32 or int64");
+  return t.to(at::kInt).contiguous();
 }
 
 // A dimension of one entry may carry any stride: it is never stepped over.
@@ -280,101 +305,138 @@ int64_t step_of(const at::Tensor& t, int64_t dim, int64_t otherwise) {
 }
 
 MasInt4KVCache int4_cache(const at::Tensor& k_codes, const at::Tensor& v_codes, const at::Tensor& pairs, bool hnd) {
-  TORCH_CHECK(k_codes.dim() == 4 && v_codes.dim() == 4 && pairs.dim() == 4 && k_codes.sizes() == v_codes.sizes(),
-              "mas_b200: k_codes and v_codes must be 4-D with identical shapes, pairs 4-D");
-  TORCH_CHECK(k_codes.scalar_type() == at::kByte && v_codes.scalar_type() == at::kByte &&
-                  pairs.scalar_type() == at::kBFloat16,
-              "mas_b200: the codes must be uint8 and the pairs bfloat16");
-  const int64_t entries = hnd ? 2 : 1, heads = hnd ? 1 : 2;
+  TORCH_CHECK_VALUE(k_codes.dim() == 4 && pairs.dim() == 4 && k_codes.sizes() == v_codes.sizes(),
+                    "k/v codes must be 4-D with identical shapes, pairs 4-D");
+  TORCH_CHECK_VALUE(k_codes.scalar_type() == at::kByte && v_codes.scalar_type() == at::kByte &&
+                        pairs.scalar_type() == at::kBFloat16,
+                    "k/v codes must be uint8 and pairs bfloat16");
+  same_device(k_codes, {&v_codes, &pairs});
+  const int64_t entries = hnd ? 2 : 1, heads = hnd ? 1 : 2, row = k_codes.size(3);
+  TORCH_CHECK_VALUE(row == 32 || row == 64, "head_dim must be 64 or 128, got ", std::to_string(2 * row));
   MasInt4KVCache c = {};
   c.k_codes = k_codes.data_ptr();
   c.v_codes = v_codes.data_ptr();
   c.pairs = pairs.data_ptr();
   c.num_pages = k_codes.size(0);
   c.page_size = k_codes.size(entries);
-  TORCH_CHECK(pairs.size(0) == c.num_pages && pairs.size(1) == k_codes.size(heads) && pairs.size(2) == c.page_size &&
-                  pairs.size(3) == 4,
-              "mas_b200: pairs must be (pages, heads, page_size, 4)");
-  const int64_t inner = pairs.size(2) * 4;
-  TORCH_CHECK(pairs.stride(3) == 1 && step_of(pairs, 2, 4) == 4 && step_of(pairs, 1, inner) == inner,
-              "mas_b200: pairs must be contiguous within a page");
-  c.pair_stride_page = step_of(pairs, 0, pairs.size(1) * inner);
-  TORCH_CHECK(k_codes.stride(3) == 1 && v_codes.stride(3) == 1,
-              "mas_b200: the codes' last dimension must be contiguous");
-  const int64_t row = k_codes.size(3);
+  TORCH_CHECK_VALUE(c.page_size > 0 && k_codes.size(heads) > 0, "page_size and the number of heads must be positive");
+  TORCH_CHECK_VALUE(pairs.size(0) == c.num_pages && pairs.size(1) == k_codes.size(heads) &&
+                        pairs.size(2) == c.page_size && pairs.size(3) == 4,
+                    "pairs must be (pages, heads, page_size, 4)");
+  const int64_t inner = c.page_size * 4, page = k_codes.size(heads) * inner;
+  TORCH_CHECK_VALUE(pairs.stride(3) == 1 && step_of(pairs, 2, 4) == 4 && step_of(pairs, 1, inner) == inner,
+                    "pairs must be contiguous within a page");
+  c.pair_stride_page = step_of(pairs, 0, page);
+  TORCH_CHECK_VALUE(c.pair_stride_page % 4 == 0 && c.pair_stride_page >= page,
+                    "pairs' pages must not overlap and lie a multiple of 4 elements apart");
   c.stride_page = step_of(k_codes, 0, row);
   c.stride_entry = step_of(k_codes, entries, row);
   c.stride_head = step_of(k_codes, heads, row);
-  TORCH_CHECK(c.stride_page == step_of(v_codes, 0, row) && c.stride_entry == step_of(v_codes, entries, row) &&
-                  c.stride_head == step_of(v_codes, heads, row),
-              "mas_b200: k_codes and v_codes must have identical strides");
+  TORCH_CHECK_VALUE(k_codes.stride(3) == 1 && v_codes.stride(3) == 1 && c.stride_page % 16 == 0 &&
+                        c.stride_entry % 16 == 0 && c.stride_head % 16 == 0,
+                    "k/v codes must be contiguous in the last dimension, the others' strides multiples of 16");
+  TORCH_CHECK_VALUE(c.stride_page == step_of(v_codes, 0, row) && c.stride_entry == step_of(v_codes, entries, row) &&
+                        c.stride_head == step_of(v_codes, heads, row),
+                    "k/v codes must have identical strides");
+  TORCH_CHECK_VALUE(reinterpret_cast<uintptr_t>(c.k_codes) % 16 == 0 && reinterpret_cast<uintptr_t>(c.v_codes) % 16 == 0 &&
+                        reinterpret_cast<uintptr_t>(c.pairs) % 8 == 0,
+                    "k/v codes must be 16-byte aligned, pairs 8-byte aligned");
   return c;
 }
 
-void allocate_paged_kv(at::Tensor append_lens, at::Tensor seq_lens, at::Tensor block_tables, at::Tensor free_pages,
-                       at::Tensor num_free, at::Tensor cum_lens, at::Tensor batch_indices, at::Tensor positions,
-                       at::Tensor last_page_len, int64_t page_size, bool enable_pdl) {
-  const c10::cuda::CUDAGuard guard(seq_lens.device());
-  const int64_t batch = seq_lens.numel();
-  check_int32(append_lens, "append_lens");
+// block_tables' row stride; seq_lens and the tables checked against each other.
+int64_t check_tables(const at::Tensor& block_tables, const at::Tensor& seq_lens) {
   check_int32(seq_lens, "seq_lens");
+  TORCH_CHECK_VALUE(block_tables.dim() == 2 && block_tables.scalar_type() == at::kInt &&
+                        block_tables.size(0) == seq_lens.numel() && step_of(block_tables, 1, 1) == 1,
+                    "block_tables must be an int32 (batch_size, max_blocks) tensor, contiguous within a row");
+  const int64_t stride = step_of(block_tables, 0, block_tables.size(1));
+  TORCH_CHECK_VALUE(stride >= block_tables.size(1), "block_tables' rows must not overlap");
+  return stride;
+}
+
+int64_t check_pages(const at::Tensor& lens, const char* name, const at::Tensor& seq_lens, const at::Tensor& block_tables,
+                    const at::Tensor& free_pages, const at::Tensor& num_free, int64_t page_size) {
+  const int64_t stride = check_tables(block_tables, seq_lens);
   check_int32(free_pages, "free_pages");
-  check_int32(num_free, "num_free");
-  check_int32(cum_lens, "cum_append_lens");
-  check_int32(batch_indices, "batch_indices");
-  check_int32(positions, "positions");
-  check_int32(last_page_len, "kv_last_page_len");
-  TORCH_CHECK(block_tables.dim() == 2 && block_tables.scalar_type() == at::kInt && block_tables.size(0) == batch &&
-                  step_of(block_tables, 1, 1) == 1,
-              "mas_b200: block_tables must be int32 (batch, max_blocks), contiguous within a row");
-  TORCH_CHECK(append_lens.numel() == batch && num_free.numel() == 1 && cum_lens.numel() == batch + 1 &&
-                  last_page_len.numel() == batch && positions.numel() == batch_indices.numel(),
-              "mas_b200: append_lens, num_free or an output has the wrong number of entries");
-  check(mas_allocate_paged_kv(append_lens.data_ptr<int32_t>(), seq_lens.data_ptr<int32_t>(),
-                              block_tables.data_ptr<int32_t>(), free_pages.data_ptr<int32_t>(),
-                              num_free.data_ptr<int32_t>(), cum_lens.data_ptr<int32_t>(),
-                              batch_indices.data_ptr<int32_t>(), positions.data_ptr<int32_t>(),
-                              last_page_len.data_ptr<int32_t>(), batch, block_tables.size(1),
-                              step_of(block_tables, 0, block_tables.size(1)), page_size, batch_indices.numel(),
-                              free_pages.numel(), nullptr, enable_pdl, stream_of(seq_lens)),
+  check_int32(num_free, "num_free", 1);
+  TORCH_CHECK_VALUE(lens.dim() == 1 && lens.numel() == seq_lens.numel(), name, " must be (batch_size,)");
+  TORCH_CHECK_VALUE(page_size > 0, "page_size must be positive");
+  TORCH_CHECK_VALUE(seq_lens.numel() <= 8192, "at most 8192 requests a call, got ", std::to_string(seq_lens.numel()));
+  same_device(seq_lens, {&lens, &block_tables, &free_pages, &num_free});
+  return stride;
+}
+
+void allocate_paged_kv_out(at::Tensor append_lens, at::Tensor seq_lens, at::Tensor block_tables, at::Tensor free_pages,
+                           at::Tensor num_free, at::Tensor cum_lens, at::Tensor batch_indices, at::Tensor positions,
+                           at::Tensor last_page_len, int64_t page_size, int64_t max_tokens, bool enable_pdl) {
+  const c10::cuda::CUDAGuard guard(seq_lens.device());
+  const int64_t stride = check_pages(append_lens, "append_lens", seq_lens, block_tables, free_pages, num_free, page_size);
+  const int64_t batch = seq_lens.numel();
+  TORCH_CHECK_VALUE(max_tokens >= 0, "max_tokens must not be negative");
+  check_int32(cum_lens, "cum_append_lens", batch + 1);
+  check_int32(batch_indices, "batch_indices", max_tokens);
+  check_int32(positions, "positions", max_tokens);
+  check_int32(last_page_len, "kv_last_page_len", batch);
+  same_device(seq_lens, {&cum_lens, &batch_indices, &positions, &last_page_len});
+  const at::Tensor lens = as_int32(append_lens, "append_lens");
+  check(mas_allocate_paged_kv(lens.data_ptr<int32_t>(), seq_lens.data_ptr<int32_t>(), block_tables.data_ptr<int32_t>(),
+                              free_pages.data_ptr<int32_t>(), num_free.data_ptr<int32_t>(),
+                              cum_lens.data_ptr<int32_t>(), batch_indices.data_ptr<int32_t>(),
+                              positions.data_ptr<int32_t>(), last_page_len.data_ptr<int32_t>(), batch,
+                              block_tables.size(1), stride, page_size, max_tokens, free_pages.numel(), nullptr,
+                              enable_pdl, stream_of(seq_lens)),
         "mas_allocate_paged_kv");
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> allocate_paged_kv(
+    at::Tensor append_lens, at::Tensor seq_lens, at::Tensor block_tables, at::Tensor free_pages, at::Tensor num_free,
+    int64_t page_size, int64_t max_tokens, bool enable_pdl) {
+  const c10::cuda::CUDAGuard guard(seq_lens.device());
+  TORCH_CHECK_VALUE(max_tokens >= 0, "max_tokens must not be negative");
+  const auto options = seq_lens.options().dtype(at::kInt);
+  at::Tensor cum = at::empty({seq_lens.numel() + 1}, options), bi = at::empty({max_tokens}, options);
+  at::Tensor pos = at::empty({max_tokens}, options), last = at::empty({seq_lens.numel()}, options);
+  allocate_paged_kv_out(append_lens, seq_lens, block_tables, free_pages, num_free, cum, bi, pos, last, page_size,
+                        max_tokens, enable_pdl);
+  return {cum, bi, pos, last};
 }
 
 void release_paged_kv(at::Tensor keep_lens, at::Tensor seq_lens, at::Tensor block_tables, at::Tensor free_pages,
                       at::Tensor num_free, int64_t page_size, bool enable_pdl) {
   const c10::cuda::CUDAGuard guard(seq_lens.device());
-  const int64_t batch = seq_lens.numel();
-  check_int32(keep_lens, "keep_lens");
-  check_int32(seq_lens, "seq_lens");
-  check_int32(free_pages, "free_pages");
-  check_int32(num_free, "num_free");
-  TORCH_CHECK(block_tables.dim() == 2 && block_tables.scalar_type() == at::kInt && block_tables.size(0) == batch &&
-                  step_of(block_tables, 1, 1) == 1,
-              "mas_b200: block_tables must be int32 (batch, max_blocks), contiguous within a row");
-  TORCH_CHECK(keep_lens.numel() == batch && num_free.numel() == 1,
-              "mas_b200: keep_lens or num_free has the wrong number of entries");
-  check(mas_release_paged_kv(keep_lens.data_ptr<int32_t>(), seq_lens.data_ptr<int32_t>(),
-                             block_tables.data_ptr<int32_t>(), free_pages.data_ptr<int32_t>(),
-                             num_free.data_ptr<int32_t>(), batch, block_tables.size(1),
-                             step_of(block_tables, 0, block_tables.size(1)), page_size, free_pages.numel(), nullptr,
-                             enable_pdl, stream_of(seq_lens)),
+  const int64_t stride = check_pages(keep_lens, "keep_lens", seq_lens, block_tables, free_pages, num_free, page_size);
+  const at::Tensor lens = as_int32(keep_lens, "keep_lens");
+  check(mas_release_paged_kv(lens.data_ptr<int32_t>(), seq_lens.data_ptr<int32_t>(), block_tables.data_ptr<int32_t>(),
+                             free_pages.data_ptr<int32_t>(), num_free.data_ptr<int32_t>(), seq_lens.numel(),
+                             block_tables.size(1), stride, page_size, free_pages.numel(), nullptr, enable_pdl,
+                             stream_of(seq_lens)),
         "mas_release_paged_kv");
 }
 
-void check_int4_rows(const at::Tensor& k, const at::Tensor& v, const at::Tensor& batch_indices,
-                     const at::Tensor& positions, const at::Tensor& k_codes, const at::Tensor& kv_indices,
-                     const at::Tensor& kv_indptr, bool hnd) {
-  TORCH_CHECK(k.dim() == 3 && v.dim() == 3 && k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type(),
-              "mas_b200: k and v must be (tokens, heads, head_size) of one dtype");
-  TORCH_CHECK(k.stride(2) == 1 && v.stride(2) == 1, "mas_b200: k and v must be contiguous in head_size");
-  check_int32(batch_indices, "batch_indices");
-  check_int32(kv_indices, "kv_indices");
-  check_int32(kv_indptr, "kv_indptr");
-  TORCH_CHECK(batch_indices.numel() == k.size(0) && positions.numel() == k.size(0) && positions.is_contiguous(),
-              "mas_b200: batch_indices and positions must be contiguous, one per token");
-  TORCH_CHECK(kv_indptr.numel() >= 1, "mas_b200: kv_indptr must have batch_size + 1 entries");
-  TORCH_CHECK(k_codes.size(hnd ? 1 : 2) == k.size(1) && 2 * k_codes.size(3) == k.size(2),
-              "mas_b200: the cache's heads/head_size differ from k's");
+// The rows of an append or a read, and the tokens they belong to.
+struct Int4Rows {
+  at::Tensor batch_indices, positions, kv_indices, kv_indptr;
+};
+
+Int4Rows int4_rows(const at::Tensor& k, const at::Tensor& v, const at::Tensor& batch_indices, const at::Tensor& positions,
+                   const at::Tensor& k_codes, const at::Tensor& kv_indices, const at::Tensor& kv_indptr, bool hnd) {
+  TORCH_CHECK_VALUE(k.dim() == 3 && v.sizes() == k.sizes() && k.scalar_type() == v.scalar_type(),
+                    "k and v must be (tokens, heads, head_dim), equal in shape and dtype");
+  TORCH_CHECK_VALUE(k.scalar_type() == at::kBFloat16 || k.scalar_type() == at::kHalf, "unsupported dtype ",
+                    k.scalar_type(), "; expected bfloat16 or float16");
+  TORCH_CHECK_VALUE(k.stride(2) == 1 && v.stride(2) == 1, "k and v must be contiguous in head_dim");
+  TORCH_CHECK_VALUE(k_codes.size(hnd ? 1 : 2) == k.size(1) && 2 * k_codes.size(3) == k.size(2),
+                    "cache heads/head_dim differ from k's");
+  TORCH_CHECK_VALUE(batch_indices.dim() == 1 && positions.dim() == 1 && batch_indices.numel() == k.size(0) &&
+                        positions.numel() == k.size(0),
+                    "batch_indices and positions must have one entry per token");
+  TORCH_CHECK_VALUE(kv_indptr.dim() == 1 && kv_indptr.numel() >= 1, "kv_indptr must have batch_size + 1 entries");
+  same_device(k, {&v, &batch_indices, &positions, &k_codes, &kv_indices, &kv_indptr});
+  TORCH_CHECK_VALUE(positions.scalar_type() == at::kInt || positions.scalar_type() == at::kLong,
+                    "positions must be int32 or int64");
+  return {as_int32(batch_indices, "batch_indices"), positions.contiguous(), as_int32(kv_indices, "kv_indices"),
+          as_int32(kv_indptr, "kv_indptr")};
 }
 
 void append_paged_kv_cache_int4(at::Tensor k, at::Tensor v, at::Tensor batch_indices, at::Tensor positions,
@@ -382,68 +444,120 @@ void append_paged_kv_cache_int4(at::Tensor k, at::Tensor v, at::Tensor batch_ind
                                 at::Tensor kv_indptr, bool hnd, bool enable_pdl) {
   const c10::cuda::CUDAGuard guard(k.device());
   const MasInt4KVCache c = int4_cache(k_codes, v_codes, pairs, hnd);
-  check_int4_rows(k, v, batch_indices, positions, k_codes, kv_indices, kv_indptr, hnd);
-  check(mas_append_paged_kv_cache_int4(k.data_ptr(), v.data_ptr(), batch_indices.data_ptr<int32_t>(),
-                                       positions.data_ptr(), id_code(positions), &c, kv_indices.data_ptr<int32_t>(),
-                                       kv_indices.numel(), kv_indptr.data_ptr<int32_t>(), kv_indptr.numel() - 1,
-                                       k.size(0), k.size(1), k.size(2), k.stride(0), k.stride(1), v.stride(0),
-                                       v.stride(1), act_code(k), nullptr, enable_pdl, stream_of(k)),
+  const Int4Rows r = int4_rows(k, v, batch_indices, positions, k_codes, kv_indices, kv_indptr, hnd);
+  check(mas_append_paged_kv_cache_int4(k.data_ptr(), v.data_ptr(), r.batch_indices.data_ptr<int32_t>(),
+                                       r.positions.data_ptr(), id_code(r.positions), &c,
+                                       r.kv_indices.data_ptr<int32_t>(), r.kv_indices.numel(),
+                                       r.kv_indptr.data_ptr<int32_t>(), r.kv_indptr.numel() - 1, k.size(0), k.size(1),
+                                       k.size(2), k.stride(0), k.stride(1), v.stride(0), v.stride(1), act_code(k),
+                                       nullptr, enable_pdl, stream_of(k)),
         "mas_append_paged_kv_cache_int4");
 }
 
-void read_paged_kv_cache_int4(at::Tensor k, at::Tensor v, at::Tensor batch_indices, at::Tensor positions,
-                              at::Tensor k_codes, at::Tensor v_codes, at::Tensor pairs, at::Tensor kv_indices,
-                              at::Tensor kv_indptr, bool hnd, bool enable_pdl) {
-  const c10::cuda::CUDAGuard guard(k.device());
+void read_paged_kv_cache_int4_out(at::Tensor k, at::Tensor v, at::Tensor batch_indices, at::Tensor positions,
+                                  at::Tensor k_codes, at::Tensor v_codes, at::Tensor pairs, at::Tensor kv_indices,
+                                  at::Tensor kv_indptr, bool hnd, bool enable_pdl) {
+  const c10::cuda::CUDAGuard guard(k_codes.device());
   const MasInt4KVCache c = int4_cache(k_codes, v_codes, pairs, hnd);
-  check_int4_rows(k, v, batch_indices, positions, k_codes, kv_indices, kv_indptr, hnd);
-  check(mas_read_paged_kv_cache_int4(k.data_ptr(), v.data_ptr(), batch_indices.data_ptr<int32_t>(),
-                                     positions.data_ptr(), id_code(positions), &c, kv_indices.data_ptr<int32_t>(),
-                                     kv_indices.numel(), kv_indptr.data_ptr<int32_t>(), kv_indptr.numel() - 1,
-                                     k.size(0), k.size(1), k.size(2), k.stride(0), k.stride(1), v.stride(0),
-                                     v.stride(1), act_code(k), nullptr, enable_pdl, stream_of(k)),
+  const Int4Rows r = int4_rows(k, v, batch_indices, positions, k_codes, kv_indices, kv_indptr, hnd);
+  check(mas_read_paged_kv_cache_int4(k.data_ptr(), v.data_ptr(), r.batch_indices.data_ptr<int32_t>(),
+                                     r.positions.data_ptr(), id_code(r.positions), &c,
+                                     r.kv_indices.data_ptr<int32_t>(), r.kv_indices.numel(),
+                                     r.kv_indptr.data_ptr<int32_t>(), r.kv_indptr.numel() - 1, k.size(0), k.size(1),
+                                     k.size(2), k.stride(0), k.stride(1), v.stride(0), v.stride(1), act_code(k), nullptr,
+                                     enable_pdl, stream_of(k)),
         "mas_read_paged_kv_cache_int4");
 }
 
-void paged_attention_int4(at::Tensor out, std::optional<at::Tensor> lse, at::Tensor q, at::Tensor k_codes,
-                          at::Tensor v_codes, at::Tensor pairs, at::Tensor block_tables, at::Tensor seq_lens,
-                          std::optional<at::Tensor> cum_seq_lens_q, double sm_scale, bool causal, bool hnd,
-                          bool enable_pdl) {
-  const c10::cuda::CUDAGuard guard(q.device());
+std::tuple<at::Tensor, at::Tensor> read_paged_kv_cache_int4(at::Tensor batch_indices, at::Tensor positions,
+                                                            at::Tensor k_codes, at::Tensor v_codes, at::Tensor pairs,
+                                                            at::Tensor kv_indices, at::Tensor kv_indptr,
+                                                            at::ScalarType dtype, bool hnd, bool enable_pdl) {
+  const c10::cuda::CUDAGuard guard(k_codes.device());
+  TORCH_CHECK_VALUE(k_codes.dim() == 4, "k/v codes must be 4-D");
+  const auto options = k_codes.options().dtype(dtype);
+  const int64_t tokens = batch_indices.numel(), heads = k_codes.size(hnd ? 1 : 2), dim = 2 * k_codes.size(3);
+  at::Tensor k = at::empty({tokens, heads, dim}, options), v = at::empty({tokens, heads, dim}, options);
+  read_paged_kv_cache_int4_out(k, v, batch_indices, positions, k_codes, v_codes, pairs, kv_indices, kv_indptr, hnd,
+                               enable_pdl);
+  return {k, v};
+}
+
+// (tokens, heads, head_dim) or (tokens, heads * head_dim) as heads and strides.
+struct HeadRows {
+  int64_t tokens, heads, stride_token, stride_head;
+};
+
+HeadRows head_rows(const at::Tensor& t, int64_t dim, const char* name) {
+  TORCH_CHECK_VALUE((t.dim() == 3 && t.size(2) == dim) || (t.dim() == 2 && t.size(1) % dim == 0), name,
+                    " must be (tokens, heads * head_dim) or (tokens, heads, head_dim) with the cache's head_dim ", std::to_string(dim));
+  TORCH_CHECK_VALUE(t.stride(-1) == 1, name, " must be contiguous in head_dim");
+  if (t.dim() == 2) return {t.size(0), t.size(1) / dim, t.stride(0), dim};
+  return {t.size(0), t.size(1), t.stride(0), t.stride(1)};
+}
+
+void paged_attention_int4_out(at::Tensor out, std::optional<at::Tensor> lse, at::Tensor query, at::Tensor k_codes,
+                              at::Tensor v_codes, at::Tensor pairs, at::Tensor block_tables, at::Tensor seq_lens,
+                              std::optional<at::Tensor> cum_seq_lens_q, std::optional<double> sm_scale, bool causal,
+                              bool hnd, bool enable_pdl) {
+  const c10::cuda::CUDAGuard guard(query.device());
   const MasInt4KVCache c = int4_cache(k_codes, v_codes, pairs, hnd);
-  const int64_t batch = seq_lens.numel();
-  TORCH_CHECK(q.dim() == 3 && out.dim() == 3 && q.sizes() == out.sizes() && q.scalar_type() == out.scalar_type() &&
-                  q.stride(2) == 1 && out.stride(2) == 1,
-              "mas_b200: query and out must be (tokens, heads, head_size) of one dtype, contiguous within a head");
-  TORCH_CHECK(q.size(2) == 2 * k_codes.size(3), "mas_b200: the cache's head_size differs from query's");
-  check_int32(seq_lens, "seq_lens");
-  TORCH_CHECK(block_tables.dim() == 2 && block_tables.scalar_type() == at::kInt && block_tables.size(0) == batch &&
-                  step_of(block_tables, 1, 1) == 1,
-              "mas_b200: block_tables must be int32 (batch, max_blocks), contiguous within a row");
+  const int64_t dim = 2 * k_codes.size(3), kv_heads = k_codes.size(hnd ? 1 : 2), batch = seq_lens.numel();
+  TORCH_CHECK_VALUE(query.scalar_type() == at::kBFloat16 || query.scalar_type() == at::kHalf, "unsupported dtype ",
+                    query.scalar_type(), "; expected bfloat16 or float16");
+  const HeadRows q = head_rows(query, dim, "query");
+  TORCH_CHECK_VALUE(q.heads > 0 && q.heads % kv_heads == 0, "query heads ", std::to_string(q.heads), " do not go with the cache's ",
+                    std::to_string(kv_heads));
+  TORCH_CHECK_VALUE(out.sizes() == query.sizes() && out.scalar_type() == query.scalar_type(),
+                    "out must have the shape and dtype of query");
+  const HeadRows o = head_rows(out, dim, "out");
+  const int64_t table_stride = check_tables(block_tables, seq_lens);
+  same_device(query, {&out, &k_codes, &block_tables, &seq_lens});
   const int32_t* cum = nullptr;
   if (cum_seq_lens_q.has_value()) {
-    check_int32(*cum_seq_lens_q, "cum_seq_lens_q");
-    TORCH_CHECK(cum_seq_lens_q->numel() == batch + 1, "mas_b200: cum_seq_lens_q must have batch_size + 1 entries");
+    check_int32(*cum_seq_lens_q, "cum_seq_lens_q", batch + 1);
+    same_device(query, {&*cum_seq_lens_q});
     cum = cum_seq_lens_q->data_ptr<int32_t>();
+  } else {
+    TORCH_CHECK_VALUE(q.tokens == batch, "without cum_seq_lens_q, query must have one row a request");
   }
+  TORCH_CHECK_VALUE(q.tokens <= INT32_MAX / q.heads, "query has more than 2^31 rows of heads");
   float* lse_ptr = nullptr;
   if (lse.has_value()) {
-    TORCH_CHECK(lse->scalar_type() == at::kFloat && lse->is_contiguous() && lse->numel() == q.size(0) * q.size(1),
-                "mas_b200: lse must be contiguous fp32 (tokens, heads)");
+    TORCH_CHECK_VALUE(lse->scalar_type() == at::kFloat && lse->is_contiguous() && lse->numel() == q.tokens * q.heads,
+                      "lse must be contiguous fp32 (tokens, heads)");
+    same_device(query, {&*lse});
     lse_ptr = lse->data_ptr<float>();
   }
-  if (batch == 0 || q.size(0) == 0) return;
+  if (batch == 0 || q.tokens == 0) return;
   // Scratch of this call alone: from the caching allocator, so a captured call keeps its own in the graph's pool.
   int64_t bytes = 0;
-  check(mas_paged_attention_int4_workspace(q.size(2), &bytes), "mas_paged_attention_int4_workspace");
-  at::Tensor work = at::empty({bytes}, q.options().dtype(at::kByte));
-  check(mas_paged_attention_int4(q.data_ptr(), out.data_ptr(), lse_ptr, &c, block_tables.data_ptr<int32_t>(),
-                                 step_of(block_tables, 0, block_tables.size(1)), block_tables.size(1),
-                                 seq_lens.data_ptr<int32_t>(), cum, batch, q.size(0), q.size(1),
-                                 k_codes.size(hnd ? 1 : 2), q.size(2), q.stride(0), q.stride(1), out.stride(0),
-                                 out.stride(1), static_cast<float>(sm_scale), causal, act_code(q), work.data_ptr(),
-                                 bytes, nullptr, enable_pdl, stream_of(q)),
+  check(mas_paged_attention_int4_workspace(dim, &bytes), "mas_paged_attention_int4_workspace");
+  at::Tensor work = at::empty({bytes}, query.options().dtype(at::kByte));
+  check(mas_paged_attention_int4(query.data_ptr(), out.data_ptr(), lse_ptr, &c, block_tables.data_ptr<int32_t>(),
+                                 table_stride, block_tables.size(1), seq_lens.data_ptr<int32_t>(), cum, batch, q.tokens,
+                                 q.heads, kv_heads, dim, q.stride_token, q.stride_head, o.stride_token, o.stride_head,
+                                 static_cast<float>(sm_scale.has_value() ? *sm_scale : 1.0 / std::sqrt((double)dim)),
+                                 causal, act_code(query), work.data_ptr(), bytes, nullptr, enable_pdl, stream_of(query)),
         "mas_paged_attention_int4");
+}
+
+std::tuple<at::Tensor, at::Tensor> paged_attention_int4(at::Tensor query, at::Tensor k_codes, at::Tensor v_codes,
+                                                        at::Tensor pairs, at::Tensor block_tables, at::Tensor seq_lens,
+                                                        std::optional<at::Tensor> cum_seq_lens_q,
+                                                        std::optional<double> sm_scale, bool causal, bool hnd,
+                                                        bool return_lse, bool enable_pdl) {
+  const c10::cuda::CUDAGuard guard(query.device());
+  TORCH_CHECK_VALUE(query.dim() == 2 || query.dim() == 3, "query must be 2-D or 3-D");
+  TORCH_CHECK_VALUE(k_codes.dim() == 4 && k_codes.size(3) > 0, "k/v codes must be 4-D");
+  at::Tensor out = at::empty(query.sizes(), query.options());
+  std::optional<at::Tensor> lse;
+  const int64_t heads = query.dim() == 3 ? query.size(1) : query.size(1) / (2 * k_codes.size(3));
+  at::Tensor held = at::empty({return_lse ? query.size(0) : 0, heads}, query.options().dtype(at::kFloat));
+  if (return_lse) lse = held;
+  paged_attention_int4_out(out, lse, query, k_codes, v_codes, pairs, block_tables, seq_lens, cum_seq_lens_q, sm_scale,
+                           causal, hnd, enable_pdl);
+  return {out, held};
 }
 
 }  // namespace
@@ -467,18 +581,26 @@ TORCH_LIBRARY(mas_b200, m) {
   m.def("embedding_out(Tensor(a!) out, Tensor input_ids, Tensor weight, bool enable_pdl) -> ()");
   m.def("embedding_fill(Tensor(a!) input_ids, Tensor weight, Tensor last_tokens, bool enable_pdl) -> Tensor");
   m.def("allocate_paged_kv(Tensor append_lens, Tensor(a!) seq_lens, Tensor(b!) block_tables, Tensor free_pages, "
+        "Tensor(c!) num_free, int page_size, int max_tokens, bool enable_pdl) -> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("allocate_paged_kv_out(Tensor append_lens, Tensor(a!) seq_lens, Tensor(b!) block_tables, Tensor free_pages, "
         "Tensor(c!) num_free, Tensor(d!) cum_append_lens, Tensor(e!) batch_indices, Tensor(f!) positions, "
-        "Tensor(g!) kv_last_page_len, int page_size, bool enable_pdl) -> ()");
+        "Tensor(g!) kv_last_page_len, int page_size, int max_tokens, bool enable_pdl) -> ()");
   m.def("release_paged_kv(Tensor keep_lens, Tensor(a!) seq_lens, Tensor block_tables, Tensor(b!) free_pages, "
         "Tensor(c!) num_free, int page_size, bool enable_pdl) -> ()");
   m.def("append_paged_kv_cache_int4(Tensor k, Tensor v, Tensor batch_indices, Tensor positions, "
         "Tensor(a!) k_codes, Tensor(b!) v_codes, Tensor(c!) pairs, Tensor kv_indices, Tensor kv_indptr, bool hnd, "
         "bool enable_pdl) -> ()");
-  m.def("read_paged_kv_cache_int4(Tensor(a!) k, Tensor(b!) v, Tensor batch_indices, Tensor positions, "
+  m.def("read_paged_kv_cache_int4(Tensor batch_indices, Tensor positions, Tensor k_codes, Tensor v_codes, "
+        "Tensor pairs, Tensor kv_indices, Tensor kv_indptr, ScalarType dtype, bool hnd, bool enable_pdl) -> "
+        "(Tensor, Tensor)");
+  m.def("read_paged_kv_cache_int4_out(Tensor(a!) k, Tensor(b!) v, Tensor batch_indices, Tensor positions, "
         "Tensor k_codes, Tensor v_codes, Tensor pairs, Tensor kv_indices, Tensor kv_indptr, bool hnd, "
         "bool enable_pdl) -> ()");
-  m.def("paged_attention_int4(Tensor(a!) out, Tensor(b!)? lse, Tensor q, Tensor k_codes, Tensor v_codes, "
-        "Tensor pairs, Tensor block_tables, Tensor seq_lens, Tensor? cum_seq_lens_q, float sm_scale, bool causal, "
+  m.def("paged_attention_int4(Tensor query, Tensor k_codes, Tensor v_codes, Tensor pairs, Tensor block_tables, "
+        "Tensor seq_lens, Tensor? cum_seq_lens_q, float? sm_scale, bool causal, bool hnd, bool return_lse, "
+        "bool enable_pdl) -> (Tensor, Tensor)");
+  m.def("paged_attention_int4_out(Tensor(a!) out, Tensor(b!)? lse, Tensor query, Tensor k_codes, Tensor v_codes, "
+        "Tensor pairs, Tensor block_tables, Tensor seq_lens, Tensor? cum_seq_lens_q, float? sm_scale, bool causal, "
         "bool hnd, bool enable_pdl) -> ()");
 }
 
@@ -495,8 +617,11 @@ TORCH_LIBRARY_IMPL(mas_b200, CUDA, m) {
   m.impl("embedding_out", &embedding_out);
   m.impl("embedding_fill", &embedding_fill);
   m.impl("allocate_paged_kv", &allocate_paged_kv);
+  m.impl("allocate_paged_kv_out", &allocate_paged_kv_out);
   m.impl("release_paged_kv", &release_paged_kv);
   m.impl("append_paged_kv_cache_int4", &append_paged_kv_cache_int4);
   m.impl("read_paged_kv_cache_int4", &read_paged_kv_cache_int4);
+  m.impl("read_paged_kv_cache_int4_out", &read_paged_kv_cache_int4_out);
   m.impl("paged_attention_int4", &paged_attention_int4);
+  m.impl("paged_attention_int4_out", &paged_attention_int4_out);
 }

@@ -23,18 +23,19 @@ c * s + m. The codes are uint8 [pages, page_size, heads, head_dim / 2] (NHD) or 
 head_dim / 2] (HND); the pairs bf16 [pages, heads, page_size, 4], (k s, k m, v s, v m), under either layout.
 At head_dim 128 that is 136 bytes a token and kv head, against 512 in 16 bits.
 
-As in ops.py, each function is a check layer over a `mas_b200::*` operator that launches on the current stream, is
-opaque to torch.compile and can be captured into a CUDA graph; there is no CPU implementation.
+As in ops.py, each function stands over a `mas_b200::*` operator that launches on the current stream, is opaque to
+torch.compile and can be captured into a CUDA graph; there is no CPU implementation. CUDA calls are checked by the operator
+itself (csrc/torch_ops.cpp), with the exceptions the checks here raise for tensors of other devices: a decode step is a few
+microseconds of kernels, and these checks took ten to twenty in Python.
 """
 from __future__ import annotations
 
-import math
 from typing import NamedTuple, Optional, Tuple
 
 import torch
 
 from . import _lib  # noqa: F401  (loads the operators)
-from .ops import _ID_DTYPES, _act_code, _check_device, _heads, _int32
+from .ops import _ID_DTYPES, _act_code, _check_device, _heads
 
 __all__ = [
     "PagedKVMaps",
@@ -50,15 +51,25 @@ MAX_REQUESTS = 8192  # a page allocation scans all lengths in one thread block's
 HEAD_DIMS = (64, 128)
 
 _OP_ALLOCATE = torch.ops.mas_b200.allocate_paged_kv.default
+_OP_ALLOCATE_OUT = torch.ops.mas_b200.allocate_paged_kv_out.default
 _OP_RELEASE = torch.ops.mas_b200.release_paged_kv.default
 _OP_APPEND = torch.ops.mas_b200.append_paged_kv_cache_int4.default
 _OP_READ = torch.ops.mas_b200.read_paged_kv_cache_int4.default
+_OP_READ_OUT = torch.ops.mas_b200.read_paged_kv_cache_int4_out.default
 _OP_ATTENTION = torch.ops.mas_b200.paged_attention_int4.default
+_OP_ATTENTION_OUT = torch.ops.mas_b200.paged_attention_int4_out.default
 
 
 @torch.library.register_fake("mas_b200::allocate_paged_kv")
+def _(append_lens, seq_lens, block_tables, free_pages, num_free, page_size, max_tokens, enable_pdl):
+    def new(n):
+        return seq_lens.new_empty((n,), dtype=torch.int32)
+    return new(seq_lens.shape[0] + 1), new(max_tokens), new(max_tokens), new(seq_lens.shape[0])
+
+
+@torch.library.register_fake("mas_b200::allocate_paged_kv_out")
 def _(append_lens, seq_lens, block_tables, free_pages, num_free, cum_append_lens, batch_indices, positions,
-      kv_last_page_len, page_size, enable_pdl) -> None:
+      kv_last_page_len, page_size, max_tokens, enable_pdl) -> None:
     return None
 
 
@@ -73,12 +84,25 @@ def _(k, v, batch_indices, positions, k_codes, v_codes, pairs, kv_indices, kv_in
 
 
 @torch.library.register_fake("mas_b200::read_paged_kv_cache_int4")
+def _(batch_indices, positions, k_codes, v_codes, pairs, kv_indices, kv_indptr, dtype, hnd, enable_pdl):
+    shape = (batch_indices.shape[0], k_codes.shape[1 if hnd else 2], 2 * k_codes.shape[3])
+    return k_codes.new_empty(shape, dtype=dtype), k_codes.new_empty(shape, dtype=dtype)
+
+
+@torch.library.register_fake("mas_b200::read_paged_kv_cache_int4_out")
 def _(k, v, batch_indices, positions, k_codes, v_codes, pairs, kv_indices, kv_indptr, hnd, enable_pdl) -> None:
     return None
 
 
 @torch.library.register_fake("mas_b200::paged_attention_int4")
-def _(out, lse, q, k_codes, v_codes, pairs, block_tables, seq_lens, cum_seq_lens_q, sm_scale, causal, hnd,
+def _(query, k_codes, v_codes, pairs, block_tables, seq_lens, cum_seq_lens_q, sm_scale, causal, hnd, return_lse, enable_pdl):
+    heads = query.shape[1] if query.dim() == 3 else query.shape[1] // (2 * k_codes.shape[3])
+    return (torch.empty(query.shape, dtype=query.dtype, device=query.device),
+            query.new_empty((query.shape[0] if return_lse else 0, heads), dtype=torch.float32))
+
+
+@torch.library.register_fake("mas_b200::paged_attention_int4_out")
+def _(out, lse, query, k_codes, v_codes, pairs, block_tables, seq_lens, cum_seq_lens_q, sm_scale, causal, hnd,
       enable_pdl) -> None:
     return None
 
@@ -97,6 +121,8 @@ def _check_tables(block_tables: torch.Tensor, seq_lens: torch.Tensor) -> int:
     if (block_tables.dim() != 2 or block_tables.dtype != torch.int32 or block_tables.shape[0] != seq_lens.shape[0]
             or (block_tables.shape[1] > 1 and block_tables.stride(1) != 1)):
         raise ValueError("block_tables must be an int32 (batch_size, max_blocks) tensor, contiguous within a row")
+    if block_tables.shape[0] > 1 and block_tables.stride(0) < block_tables.shape[1]:
+        raise ValueError("block_tables' rows must not overlap")
     return seq_lens.shape[0]
 
 
@@ -122,8 +148,6 @@ def _check_pages(seq_lens, block_tables, free_pages, num_free, page_size) -> int
         raise ValueError("page_size must be positive")
     if batch > MAX_REQUESTS:
         raise ValueError(f"at most {MAX_REQUESTS} requests a call, got {batch}")
-    if batch > 1 and block_tables.stride(0) < block_tables.shape[1]:
-        raise ValueError("block_tables' rows must not overlap")
     return batch
 
 
@@ -142,24 +166,26 @@ def allocate_paged_kv(append_lens: torch.Tensor, seq_lens: torch.Tensor, block_t
     stays as it is, the maps say that no token has a place, and STATUS_KV_ALLOC_REFUSED is set in the device
     status word (`read_status`). At most 8192 requests.
     """
+    pdl = True if enable_pdl is None else bool(enable_pdl)
+    if not seq_lens.is_cuda:
+        _check_allocate(append_lens, seq_lens, block_tables, free_pages, num_free, page_size, max_tokens, out)
+    if out is None:
+        return PagedKVMaps(*_OP_ALLOCATE(append_lens, seq_lens, block_tables, free_pages, num_free, page_size, max_tokens, pdl))
+    _OP_ALLOCATE_OUT(append_lens, seq_lens, block_tables, free_pages, num_free, *out, page_size, max_tokens, pdl)
+    return PagedKVMaps(*out)
+
+
+def _check_allocate(append_lens, seq_lens, block_tables, free_pages, num_free, page_size, max_tokens, out) -> None:
     batch = _check_pages(seq_lens, block_tables, free_pages, num_free, page_size)
     if append_lens.shape != (batch,) or append_lens.dtype not in _ID_DTYPES:
         raise ValueError("append_lens must be an int32 or int64 (batch_size,) tensor")
     if max_tokens < 0:
         raise ValueError("max_tokens must not be negative")
-    if out is None:
-        def new(n):
-            return torch.empty((n,), dtype=torch.int32, device=seq_lens.device)
-        out = PagedKVMaps(new(batch + 1), new(max_tokens), new(max_tokens), new(batch))
-    else:
-        out = PagedKVMaps(*out)
-        for name, t, n in zip(PagedKVMaps._fields, out, (batch + 1, max_tokens, max_tokens, batch)):
-            _check_int32(name, t, (n,))
+    maps = {} if out is None else PagedKVMaps(*out)._asdict()
+    for (name, t), n in zip(maps.items(), (batch + 1, max_tokens, max_tokens, batch)):
+        _check_int32(name, t, (n,))
     _check_device(seq_lens, append_lens=append_lens, block_tables=block_tables, free_pages=free_pages,
-                  num_free=num_free, **out._asdict())
-    _OP_ALLOCATE(_int32(append_lens), seq_lens, block_tables, free_pages, num_free, *out, int(page_size),
-                 True if enable_pdl is None else bool(enable_pdl))
-    return out
+                  num_free=num_free, **maps)
 
 
 def release_paged_kv(keep_lens: torch.Tensor, seq_lens: torch.Tensor, block_tables: torch.Tensor,
@@ -172,11 +198,12 @@ def release_paged_kv(keep_lens: torch.Tensor, seq_lens: torch.Tensor, block_tabl
     requests share must not be released through each of them. A call that does not fit changes nothing and sets
     STATUS_KV_ALLOC_REFUSED.
     """
-    batch = _check_pages(seq_lens, block_tables, free_pages, num_free, page_size)
-    if keep_lens.shape != (batch,) or keep_lens.dtype not in _ID_DTYPES:
-        raise ValueError("keep_lens must be an int32 or int64 (batch_size,) tensor")
-    _check_device(seq_lens, keep_lens=keep_lens, block_tables=block_tables, free_pages=free_pages, num_free=num_free)
-    _OP_RELEASE(_int32(keep_lens), seq_lens, block_tables, free_pages, num_free, int(page_size),
+    if not seq_lens.is_cuda:
+        batch = _check_pages(seq_lens, block_tables, free_pages, num_free, page_size)
+        if keep_lens.shape != (batch,) or keep_lens.dtype not in _ID_DTYPES:
+            raise ValueError("keep_lens must be an int32 or int64 (batch_size,) tensor")
+        _check_device(seq_lens, keep_lens=keep_lens, block_tables=block_tables, free_pages=free_pages, num_free=num_free)
+    _OP_RELEASE(keep_lens, seq_lens, block_tables, free_pages, num_free, page_size,
                 True if enable_pdl is None else bool(enable_pdl))
 
 
@@ -186,28 +213,34 @@ def release_paged_kv(keep_lens: torch.Tensor, seq_lens: torch.Tensor, block_tabl
 def empty_paged_kv_cache_int4(num_pages: int, page_size: int, num_kv_heads: int, head_dim: int,
                               kv_layout: str = "NHD", device="cuda") -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """One layer's cache, (k_codes, v_codes, pairs), all zeros: every row reads as zeros."""
-    if kv_layout not in ("NHD", "HND"):
-        raise KeyError(f"Invalid kv_layout {kv_layout}")
+    hnd = _is_hnd(kv_layout)
     if head_dim not in HEAD_DIMS:
         raise ValueError(f"head_dim must be one of {HEAD_DIMS}, got {head_dim}")
-    inner = (page_size, num_kv_heads) if kv_layout == "NHD" else (num_kv_heads, page_size)
+    inner = (page_size, num_kv_heads) if not hnd else (num_kv_heads, page_size)
     codes = [torch.zeros((num_pages, *inner, head_dim // 2), dtype=torch.uint8, device=device) for _ in range(2)]
     return codes[0], codes[1], torch.zeros((num_pages, num_kv_heads, page_size, 4), dtype=torch.bfloat16, device=device)
 
 
-def _unpack_cache(paged_kv_cache, kv_layout: str):
-    """(k_codes, v_codes, pairs, heads, head_dim), checked."""
+def _is_hnd(kv_layout: str) -> bool:
     if kv_layout not in ("NHD", "HND"):
         raise KeyError(f"Invalid kv_layout {kv_layout}")
+    return kv_layout == "HND"
+
+
+def _parts(paged_kv_cache):
     if not isinstance(paged_kv_cache, (tuple, list)) or len(paged_kv_cache) != 3:
         raise KeyError("paged_kv_cache must be (k_codes, v_codes, pairs)")
-    k_codes, v_codes, pairs = paged_kv_cache
+    return paged_kv_cache
+
+
+def _check_cache(k_codes, v_codes, pairs, hnd: bool):
+    """(heads, head_dim) of a cache whose layout the kernels take."""
     if k_codes.dim() != 4 or k_codes.shape != v_codes.shape:
         raise ValueError("k/v codes must be 4-D with identical shapes")
     if k_codes.dtype != torch.uint8 or v_codes.dtype != torch.uint8 or pairs.dtype != torch.bfloat16:
         raise ValueError("k/v codes must be uint8 and pairs bfloat16")
     pages, page_size, heads = k_codes.shape[0], k_codes.shape[1], k_codes.shape[2]
-    if kv_layout == "HND":
+    if hnd:
         page_size, heads = heads, page_size
     head_dim = 2 * k_codes.shape[3]
     if head_dim not in HEAD_DIMS:
@@ -227,19 +260,17 @@ def _unpack_cache(paged_kv_cache, kv_layout: str):
                 raise ValueError("k/v codes must have identical strides")
             if k_codes.stride(n) % 16 if n < 3 else k_codes.stride(n) != 1:
                 raise ValueError("k/v codes must be contiguous in the last dimension, the others' strides multiples of 16")
-    for name, t, n in (("k codes", k_codes, 16), ("v codes", v_codes, 16), ("pairs", pairs, 8)):
-        if t.device.type == "cuda" and t.data_ptr() % n:
-            raise ValueError(f"the {name} must be {n}-byte aligned")
     _check_device(k_codes, v_codes=v_codes, pairs=pairs)
-    return k_codes, v_codes, pairs, heads, head_dim
+    return heads, head_dim
 
 
-def _check_rows(batch_indices, positions, kv_indptr, tokens: int) -> torch.Tensor:
+def _check_rows(batch_indices, positions, kv_indptr, tokens: int) -> None:
     if batch_indices.shape != (tokens,) or positions.shape != (tokens,):
         raise ValueError("batch_indices and positions must have one entry per token")
     if kv_indptr.dim() != 1 or kv_indptr.shape[0] < 1:
         raise ValueError("kv_indptr must have batch_size + 1 entries")
-    return (positions if positions.dtype in _ID_DTYPES else positions.int()).contiguous()
+    if positions.dtype not in _ID_DTYPES:
+        raise ValueError("positions must be int32 or int64")
 
 
 def append_paged_kv_cache_int4(append_key: torch.Tensor, append_value: torch.Tensor, batch_indices: torch.Tensor,
@@ -255,26 +286,26 @@ def append_paged_kv_cache_int4(append_key: torch.Tensor, append_value: torch.Ten
     fp32; a row that holds a NaN or an infinity reads as NaN. A token with ``batch_indices[i] == -1`` (the padding that
     `allocate_paged_kv` leaves) is skipped. Two tokens must not name one slot. head_dim is 64 or 128.
     """
-    k_codes, v_codes, pairs, heads, head_dim = _unpack_cache(paged_kv_cache, kv_layout)
-    if append_key.dim() != 3 or append_value.shape != append_key.shape:
-        raise ValueError("append_key and append_value must be (nnz, num_kv_heads, head_dim) and equal in shape")
-    if append_key.dtype != append_value.dtype:
-        raise ValueError("append_key and append_value must share one dtype")
-    _act_code(append_key)
-    if tuple(append_key.shape[1:]) != (heads, head_dim):
-        raise ValueError(f"cache heads/head_dim {(heads, head_dim)} differ from {tuple(append_key.shape[1:])}")
-    if append_key.stride(2) != 1 or append_value.stride(2) != 1:
-        raise ValueError("append_key and append_value must be contiguous in head_dim")
-    nnz = append_key.shape[0]
-    positions = _check_rows(batch_indices, positions, kv_indptr, nnz)
-    if kv_last_page_len.dim() != 1 or kv_indptr.shape[0] != kv_last_page_len.shape[0] + 1:
+    hnd = _is_hnd(kv_layout)
+    k_codes, v_codes, pairs = _parts(paged_kv_cache)
+    if kv_last_page_len.dim() != 1 or kv_indptr.dim() != 1 or kv_indptr.shape[0] != kv_last_page_len.shape[0] + 1:
         raise ValueError("kv_indptr must have batch_size + 1 entries, kv_last_page_len batch_size")
-    _check_device(append_key, append_value=append_value, batch_indices=batch_indices, positions=positions,
-                  k_codes=k_codes, kv_indices=kv_indices, kv_indptr=kv_indptr)
-    if nnz == 0:
-        return
-    _OP_APPEND(append_key, append_value, _int32(batch_indices), positions, k_codes, v_codes, pairs, _int32(kv_indices),
-               _int32(kv_indptr), kv_layout == "HND", True if enable_pdl is None else bool(enable_pdl))
+    if not append_key.is_cuda:
+        heads, head_dim = _check_cache(k_codes, v_codes, pairs, hnd)
+        if append_key.dim() != 3 or append_value.shape != append_key.shape:
+            raise ValueError("append_key and append_value must be (nnz, num_kv_heads, head_dim) and equal in shape")
+        if append_key.dtype != append_value.dtype:
+            raise ValueError("append_key and append_value must share one dtype")
+        _act_code(append_key)
+        if tuple(append_key.shape[1:]) != (heads, head_dim):
+            raise ValueError(f"cache heads/head_dim {(heads, head_dim)} differ from {tuple(append_key.shape[1:])}")
+        if append_key.stride(2) != 1 or append_value.stride(2) != 1:
+            raise ValueError("append_key and append_value must be contiguous in head_dim")
+        _check_rows(batch_indices, positions, kv_indptr, append_key.shape[0])
+        _check_device(append_key, append_value=append_value, batch_indices=batch_indices, positions=positions,
+                      k_codes=k_codes, kv_indices=kv_indices, kv_indptr=kv_indptr)
+    _OP_APPEND(append_key, append_value, batch_indices, positions, k_codes, v_codes, pairs, kv_indices, kv_indptr, hnd,
+               True if enable_pdl is None else bool(enable_pdl))
 
 
 def read_paged_kv_cache_int4(batch_indices: torch.Tensor, positions: torch.Tensor, paged_kv_cache,
@@ -288,15 +319,26 @@ def read_paged_kv_cache_int4(batch_indices: torch.Tensor, positions: torch.Tenso
     kernel of another library, a check, a copy to a 16-bit cache. A padding row (-1) or one out of range (flagged as
     in the append) reads as zeros. `out` takes two tensors that share shape and dtype (any strides, contiguous in head_dim).
     """
-    k_codes, v_codes, pairs, heads, head_dim = _unpack_cache(paged_kv_cache, kv_layout)
-    nnz = batch_indices.shape[0]
-    positions = _check_rows(batch_indices, positions, kv_indptr, nnz)
+    hnd = _is_hnd(kv_layout)
+    k_codes, v_codes, pairs = _parts(paged_kv_cache)
+    pdl = True if enable_pdl is None else bool(enable_pdl)
+    if out is None and dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"unsupported dtype {dtype}; expected bfloat16 or float16")
+    if not k_codes.is_cuda:
+        _check_read(batch_indices, positions, k_codes, v_codes, pairs, kv_indices, kv_indptr, hnd, out)
     if out is None:
-        if dtype not in (torch.bfloat16, torch.float16):
-            raise ValueError(f"unsupported dtype {dtype}; expected bfloat16 or float16")
-        key, value = (torch.empty((nnz, heads, head_dim), dtype=dtype, device=k_codes.device) for _ in range(2))
-    else:
-        key, value = out
+        return _OP_READ(batch_indices, positions, k_codes, v_codes, pairs, kv_indices, kv_indptr, dtype, hnd, pdl)
+    key, value = out
+    _OP_READ_OUT(key, value, batch_indices, positions, k_codes, v_codes, pairs, kv_indices, kv_indptr, hnd, pdl)
+    return key, value
+
+
+def _check_read(batch_indices, positions, k_codes, v_codes, pairs, kv_indices, kv_indptr, hnd, out) -> None:
+    heads, head_dim = _check_cache(k_codes, v_codes, pairs, hnd)
+    nnz = batch_indices.shape[0]
+    _check_rows(batch_indices, positions, kv_indptr, nnz)
+    key, value = (None, None) if out is None else out
+    if out is not None:
         if tuple(key.shape) != (nnz, heads, head_dim) or value.shape != key.shape:
             raise ValueError(f"out must be two {(nnz, heads, head_dim)} tensors")
         if key.dtype != value.dtype:
@@ -306,10 +348,6 @@ def read_paged_kv_cache_int4(batch_indices: torch.Tensor, positions: torch.Tenso
             raise ValueError("out must be contiguous in head_dim")
     _check_device(k_codes, batch_indices=batch_indices, positions=positions, kv_indices=kv_indices, kv_indptr=kv_indptr,
                   key=key, value=value)
-    if nnz:
-        _OP_READ(key, value, _int32(batch_indices), positions, k_codes, v_codes, pairs, _int32(kv_indices),
-                 _int32(kv_indptr), kv_layout == "HND", True if enable_pdl is None else bool(enable_pdl))
-    return key, value
 
 
 # ------------------------------------------------------------------------------------------------
@@ -335,7 +373,26 @@ def paged_attention_int4(query: torch.Tensor, paged_kv_cache, block_tables: torc
     partial attentions takes it. A page id out of range reads as zeros and lengths that do not fit the table or
     `query` are cut to them; both set STATUS_KV_SLOT_OUT_OF_RANGE.
     """
-    k_codes, v_codes, pairs, kv_heads, head_dim = _unpack_cache(paged_kv_cache, kv_layout)
+    hnd = _is_hnd(kv_layout)
+    k_codes, v_codes, pairs = _parts(paged_kv_cache)
+    pdl = True if enable_pdl is None else bool(enable_pdl)
+    if not query.is_cuda:
+        _check_attention(query, k_codes, v_codes, pairs, block_tables, seq_lens, cum_seq_lens_q, hnd, out)
+    if out is None:
+        out, lse = _OP_ATTENTION(query, k_codes, v_codes, pairs, block_tables, seq_lens, cum_seq_lens_q, sm_scale, causal, hnd,
+                                 return_lse, pdl)
+    else:
+        lse = None
+        if return_lse:
+            heads = query.shape[1] if query.dim() == 3 else query.shape[1] // (2 * k_codes.shape[3])
+            lse = torch.empty((query.shape[0], heads), dtype=torch.float32, device=query.device)
+        _OP_ATTENTION_OUT(out, lse, query, k_codes, v_codes, pairs, block_tables, seq_lens, cum_seq_lens_q, sm_scale, causal,
+                          hnd, pdl)
+    return (out, lse) if return_lse else out
+
+
+def _check_attention(query, k_codes, v_codes, pairs, block_tables, seq_lens, cum_seq_lens_q, hnd, out) -> None:
+    kv_heads, head_dim = _check_cache(k_codes, v_codes, pairs, hnd)
     q = _heads(query, head_dim)
     _act_code(q)
     if q.shape[2] != head_dim or q.shape[1] == 0 or q.shape[1] % kv_heads:
@@ -348,17 +405,6 @@ def paged_attention_int4(query: torch.Tensor, paged_kv_cache, block_tables: torc
             raise ValueError("without cum_seq_lens_q, query must have one row a request")
     else:
         _check_int32("cum_seq_lens_q", cum_seq_lens_q, (batch + 1,))
-    if q.shape[0] * q.shape[1] >= 1 << 31:
-        raise ValueError("query has more than 2^31 rows of heads")
-    if out is None:
-        out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-    elif out.shape != query.shape or out.dtype != query.dtype or out.stride(-1) != 1:
+    if out is not None and (out.shape != query.shape or out.dtype != query.dtype or out.stride(-1) != 1):
         raise ValueError("out must have the shape and dtype of query and be contiguous in head_dim")
-    o = _heads(out, head_dim)
-    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
     _check_device(q, k_codes=k_codes, block_tables=block_tables, seq_lens=seq_lens, cum_seq_lens_q=cum_seq_lens_q, out=out)
-    if q.shape[0] and batch:
-        _OP_ATTENTION(o, lse, q, k_codes, v_codes, pairs, block_tables, seq_lens, cum_seq_lens_q,
-                      1.0 / math.sqrt(head_dim) if sm_scale is None else float(sm_scale), bool(causal),
-                      kv_layout == "HND", True if enable_pdl is None else bool(enable_pdl))
-    return (out, lse) if return_lse else out

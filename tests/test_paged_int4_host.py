@@ -84,7 +84,7 @@ def t(*shape, dtype=I32, device=M):
     return torch.empty(shape, dtype=dtype, device=device)
 
 
-@pytest.mark.parametrize("fn,kw,exc", [
+REFUSALS = [
     (_append, dict(kv_layout="NDH"), KeyError),
     (_append, dict(paged_kv_cache=_cache()[:2]), KeyError),
     (_append, dict(append_value=t(3, 2, 64, dtype=BF)), ValueError),
@@ -131,10 +131,35 @@ def t(*shape, dtype=I32, device=M):
     (_release, dict(keep_lens=t(1)), ValueError),
     (_release, dict(block_tables=t(2, 5, dtype=torch.int64)), ValueError),
     (_release, dict(num_free=t(1, device="cpu")), RuntimeError),
-])
+]
+
+
+@pytest.mark.parametrize("fn,kw,exc", REFUSALS)
 def test_refusals(fn, kw, exc):
     with pytest.raises(exc):
         fn(**kw)
+
+
+def _onto(x, device):
+    """Meta tensors as tensors of that layout on `device`; others as they are."""
+    if torch.is_tensor(x):
+        return torch.empty_strided(x.shape, x.stride(), dtype=x.dtype, device=device) if x.device.type == "meta" else x
+    return tuple(_onto(y, device) for y in x) if isinstance(x, tuple) else x
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fn,kw,exc", REFUSALS)
+def test_refusals_of_cuda_calls(cuda, monkeypatch, fn, kw, exc):
+    """The operators' own checks of CUDA tensors raise what the Python checks raise; nothing is launched."""
+    import mas_b200.paged_int4 as module
+
+    for name in ("append_paged_kv_cache_int4", "read_paged_kv_cache_int4", "paged_attention_int4", "allocate_paged_kv",
+                 "release_paged_kv"):
+        real = getattr(module, name)
+        monkeypatch.setattr(mas_b200, name, lambda real=real, **a: real(**{k: _onto(v, cuda) for k, v in a.items()}))
+    with pytest.raises(exc):
+        fn(**kw)
+    torch.cuda.synchronize()
 
 
 def test_no_cpu_implementation():
