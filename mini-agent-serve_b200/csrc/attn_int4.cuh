@@ -184,18 +184,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return y;
 }
 
-__device__ __forceinline__ float2 add2_f32(float2 a, float2 b) {
-  float2 c;
-  asm("{\n\t.reg .b64 ra, rb, rc;\n\t"
-      "mov.b64 ra, {%2, %3};\n\t"
-      "mov.b64 rb, {%4, %5};\n\t"
-      "add.rn.f32x2 rc, ra, rb;\n\t"
-      "mov.b64 {%0, %1}, rc;\n\t}"
-      : "=f"(c.x), "=f"(c.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return c;
-}
-__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 __device__ __forceinline__ uint32_t max_nan_half2(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));

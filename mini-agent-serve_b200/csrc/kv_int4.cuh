@@ -91,6 +91,45 @@ __device__ __forceinline__ KVSlot kv_int4_slot(const KVInt4RowArgs& a, int64_t t
 constexpr int kKVInt4Threads = 256;
 constexpr int kKVInt4Unroll = 4;  // row pairs a warp holds at once
 
+// Packed 16-bit minima and maxima that pass a NaN on.
+template <typename T>
+__device__ __forceinline__ uint32_t min2_nan(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if (std::is_same<T, __half>::value) asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if (std::is_same<T, __half>::value) asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ float2 add2_rz_f32(float2 a, float2 b) {
+  float2 c;
+  asm("{\n\t.reg .b64 ra, rb, rc;\n\t"
+      "mov.b64 ra, {%2, %3};\n\t"
+      "mov.b64 rb, {%4, %5};\n\t"
+      "add.rz.f32x2 rc, ra, rb;\n\t"
+      "mov.b64 {%0, %1}, rc;\n\t}"
+      : "=f"(c.x), "=f"(c.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return c;
+}
+__device__ __forceinline__ float2 add2_f32(float2 a, float2 b) {
+  float2 c;
+  asm("{\n\t.reg .b64 ra, rb, rc;\n\t"
+      "mov.b64 ra, {%2, %3};\n\t"
+      "mov.b64 rb, {%4, %5};\n\t"
+      "add.rn.f32x2 rc, ra, rb;\n\t"
+      "mov.b64 {%0, %1}, rc;\n\t}"
+      : "=f"(c.x), "=f"(c.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return c;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
 // 8 consecutive elements of a row as four packed words.
 template <bool ALIGNED>
 __device__ __forceinline__ Vec16 kv_load8(const uint16_t* p) {
@@ -153,38 +192,33 @@ __global__ void __launch_bounds__(kKVInt4Threads) append_kv_int4_kernel(const KV
 #pragma unroll
     for (int i = 0; i < kKVInt4Unroll; ++i) {
       const int h = head0 + i * kHeads;
-      float f[8];
-      unpack8<T>(x[i], f);
-      float lo = f[0], hi = f[0];
-      // x * 0 is NaN for a NaN or an infinity and 0 otherwise: the sum over the row tells them apart.
-      float odd = 0.0f;
+      const uint32_t xs[4] = {x[i].a, x[i].b, x[i].c, x[i].d};
+      uint32_t lo2 = min2_nan<T>(min2_nan<T>(xs[0], xs[1]), min2_nan<T>(xs[2], xs[3]));
+      uint32_t hi2 = max2_nan<T>(max2_nan<T>(xs[0], xs[1]), max2_nan<T>(xs[2], xs[3]));
+      // The minimum and the negated maximum travel as one pair: a single minimum reduces both.
+      lo2 = min2_nan<T>(lo2, __byte_perm(lo2, lo2, 0x1032));
+      hi2 = max2_nan<T>(hi2, __byte_perm(hi2, hi2, 0x1032));
+      uint32_t ends = __byte_perm(lo2, hi2 ^ 0x80008000u, 0x5410);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        lo = fminf(lo, f[j]);
-        hi = fmaxf(hi, f[j]);
-        odd = fmaf(f[j], 0.0f, odd);
-      }
-#pragma unroll
-      for (int o = kLanes / 2; o > 0; o >>= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        odd += __shfl_xor_sync(0xffffffffu, odd, o);
-      }
-      const bool finite = odd == 0.0f;
+      for (int o = kLanes / 2; o > 0; o >>= 1) ends = min2_nan<T>(ends, __shfl_xor_sync(0xffffffffu, ends, o));
+      const float2 lh = Elem<T>::to_f2(ends);
+      const float lo = lh.x, hi = -lh.y;
+      const bool finite = fabsf(lo) <= 3.4e38f && fabsf(hi) <= 3.4e38f;
       const float m = kv_min_down(lo);
       const float nmh = -0.5f * m;
       const float s = kv_scale_up(__fmaf_ru(hi, 0.5f, nmh));
       const float sh = 0.5f * s, inv = __frcp_rn(sh);
+      // word accumulates bits(big) + 1 - (r < 0), whose low digit is the code; the constant digits leave at the end.
       uint32_t word = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float d = __fmaf_rn(f[j], 0.5f, nmh);
-        const float big = __fadd_rz(__fmul_rn(d, inv), 8388608.0f);  // floor, in the low bits
-        const float c0 = big - 8388608.0f;
-        const float r = fmaf(-(c0 + 0.5f), sh, d);
-        const uint32_t c = (__float_as_uint(big) & 31u) + (r >= 0.0f ? 1u : 0u);
-        word |= c << (4 * j);
+      for (int j = 3; j >= 0; --j) {
+        const float2 d = fma2_f32(Elem<T>::to_f2(xs[j]), both(0.5f), both(nmh));
+        const float2 big = add2_rz_f32(mul2_f32(d, both(inv)), both(8388608.0f));  // 2^23 + c0
+        const float2 r = fma2_f32(add2_f32(big, both(-8388607.5f)), both(-sh), d);
+        word = word * 16u + __float_as_uint(big.y) - (__float_as_uint(r.y) >> 31);
+        word = word * 16u + __float_as_uint(big.x) - (__float_as_uint(r.x) >> 31);
       }
+      word -= (0x4b000000u - 1u) * 0x11111111u;
       if (h < a.kv.heads) {
         *reinterpret_cast<uint32_t*>(codes + (int64_t)h * a.kv.stride_head) = finite ? word : 0u;
         if (col == 0) {
@@ -197,13 +231,10 @@ __global__ void __launch_bounds__(kKVInt4Threads) append_kv_int4_kernel(const KV
   pdl_launch_dependents();
 }
 
-// A value of the cache in T: c * s + m of a row that ends near T's largest value may lie a step past it, and reads
-// as that value.
+// T's largest value: c * s + m of a row that ends near it may lie a step past it, and reads as that value.
 template <typename T>
-__device__ __forceinline__ float kv_in_range(float x) {
-  const float top = Elem<T>::to_f(std::is_same<T, __half>::value ? 0x7bff : 0x7f7f);
-  x = x > top ? top : x;
-  return x < -top ? -top : x;
+__device__ __forceinline__ float kv_top() {
+  return std::is_same<T, __half>::value ? 65504.0f : 3.38953139e38f;
 }
 
 // The read-back: the same lanes, 4 bytes of codes in and 16 bytes of values out each.
@@ -243,7 +274,22 @@ __global__ void __launch_bounds__(kKVInt4Threads) read_kv_int4_kernel(const KVIn
       const float s = __uint_as_float(pair[i] << 16), m = __uint_as_float(pair[i] & 0xffff0000u);
       float f[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = kv_in_range<T>(fmaf((float)((word[i] >> (4 * j)) & 15u), s, m));
+      for (int j = 0; j < 8; j += 2) {
+        // 16 + c, the code in the top of the mantissa
+        const uint32_t c0 = (j < 5 ? word[i] << (19 - 4 * j) : word[i] >> (4 * j - 19)) & 0x780000u;
+        const uint32_t c1 = (j < 4 ? word[i] << (15 - 4 * j) : word[i] >> (4 * j - 15)) & 0x780000u;
+        const float2 c = add2_f32(make_float2(__uint_as_float(c0 | 0x41800000u), __uint_as_float(c1 | 0x41800000u)), both(-16.0f));
+        const float2 v = fma2_f32(c, both(s), both(m));
+        f[j] = v.x;
+        f[j + 1] = v.y;
+      }
+      if (fmaf(15.0f, s, m) > kv_top<T>() || m < -kv_top<T>()) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          f[j] = f[j] > kv_top<T>() ? kv_top<T>() : f[j];
+          f[j] = f[j] < -kv_top<T>() ? -kv_top<T>() : f[j];
+        }
+      }
       kv_store8<ALIGNED>(row + (int64_t)h * (is_v ? a.vsh : a.ksh), pack8<T>(f));
     }
   }

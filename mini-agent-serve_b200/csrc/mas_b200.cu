@@ -609,8 +609,11 @@ template <bool RELEASE>
 int launch_alloc(AllocArgs a, int64_t outputs, DeviceState* st, void* stream, int enable_pdl) {
   if (a.status == nullptr) a.status = st->status;
   const size_t smem = 3 * sizeof(int32_t) * (size_t)(a.B + 1);
-  if (outputs <= kAllocSingleOutputs)
-    return launch(paged_alloc_kernel<RELEASE, false>, dim3(1), dim3(kAllocThreads), smem, stream, enable_pdl, a);
+  if (outputs <= kAllocSingleOutputs) {
+    const bool small = a.B <= kAllocSmallThreads && outputs <= 4 * kAllocSmallThreads;
+    return launch(paged_alloc_kernel<RELEASE, false>, dim3(1), dim3(small ? kAllocSmallThreads : kAllocThreads), smem,
+                  stream, enable_pdl, a);
+  }
   return launch_cluster(paged_alloc_kernel<RELEASE, true>, dim3(kAllocClusterCtas), dim3(kAllocThreads),
                         kAllocClusterCtas, smem, stream, enable_pdl, a);
 }
