@@ -44,6 +44,7 @@ struct KVInt4RowArgs {
   int64_t num_indices;
   const int32_t* kv_indptr;
   int64_t batch_size;
+  int32_t page_shift;            // log2(page_size), or -1
   const int32_t* batch_indices;  // [T]; -1: a padding row
   const void* pos;               // [T]
   int64_t T;
@@ -77,15 +78,17 @@ struct KVSlot {
 
 template <typename PosT>
 __device__ __forceinline__ KVSlot kv_int4_slot(const KVInt4RowArgs& a, int64_t t) {
-  const int64_t b = a.batch_indices[t], pos = (int64_t)static_cast<const PosT*>(a.pos)[t];
+  const int32_t b = a.batch_indices[t];
+  const int64_t pos = (int64_t)static_cast<const PosT*>(a.pos)[t];
   if (b == -1) return {0, -2};
-  if (b < 0 || b >= a.batch_size || pos < 0) return {0, -1};
+  if (b < 0 || b >= a.batch_size || pos < 0 || pos > INT32_MAX) return {0, -1};
   const int64_t first = a.kv_indptr[b];
-  const int64_t block = pos / a.kv.page_size;
+  const uint32_t p = (uint32_t)pos, size = (uint32_t)a.kv.page_size;
+  const uint32_t block = a.page_shift >= 0 ? p >> a.page_shift : p / size;
   if (first < 0 || first + block >= a.num_indices) return {0, -1};
   const int64_t page = a.kv_indices[first + block];
   if (page < 0 || page >= a.kv.num_pages) return {0, -1};
-  return {page, (int32_t)(pos - block * a.kv.page_size)};
+  return {page, (int32_t)(p - block * size)};
 }
 
 constexpr int kKVInt4Threads = 256;
@@ -157,7 +160,8 @@ __device__ __forceinline__ void kv_store8(uint16_t* p, const Vec16& v) {
 
 // One pass of a warp stores 32 / (D / 8) rows (the k and the v row of one head at D = 128, of two at 64),
 // 8 elements a lane, so a row's minimum and maximum are a few shuffles away and its codes leave as one
-// 4-byte word a lane. A warp takes up to kKVInt4Unroll passes of one token, all their loads first.
+// 4-byte word a lane. A warp takes up to kKVInt4Unroll passes of one token, all their loads first
+// (grid: x over tokens, y over its groups of heads, so that no index is divided).
 template <typename T, typename PosT, int D, bool ALIGNED>
 __global__ void __launch_bounds__(kKVInt4Threads) append_kv_int4_kernel(const KVInt4RowArgs a) {
   constexpr int kLanes = D / 8;               // lanes a row
@@ -167,12 +171,9 @@ __global__ void __launch_bounds__(kKVInt4Threads) append_kv_int4_kernel(const KV
   const int lane = threadIdx.x & 31;
   const int sub = lane / kLanes, col = lane % kLanes;
   const bool is_v = sub & 1;
-  const int groups = (a.kv.heads + kGroup - 1) / kGroup;
-  const int64_t units = a.T * groups;
+  const int head0 = blockIdx.y * kGroup + (sub >> 1);
   const int64_t nwarps = ((int64_t)gridDim.x * kKVInt4Threads) >> 5;
-  for (int64_t u = ((int64_t)blockIdx.x * kKVInt4Threads + threadIdx.x) >> 5; u < units; u += nwarps) {
-    const int64_t t = u / groups;
-    const int head0 = (int)(u - t * groups) * kGroup + (sub >> 1);
+  for (int64_t t = ((int64_t)blockIdx.x * kKVInt4Threads + threadIdx.x) >> 5; t < a.T; t += nwarps) {
     const uint16_t* row = static_cast<const uint16_t*>(is_v ? a.v : a.k) + t * (is_v ? a.vsn : a.ksn) + col * 8;
     Vec16 x[kKVInt4Unroll];
 #pragma unroll
@@ -247,12 +248,9 @@ __global__ void __launch_bounds__(kKVInt4Threads) read_kv_int4_kernel(const KVIn
   const int lane = threadIdx.x & 31;
   const int sub = lane / kLanes, col = lane % kLanes;
   const bool is_v = sub & 1;
-  const int groups = (a.kv.heads + kGroup - 1) / kGroup;
-  const int64_t units = a.T * groups;
+  const int head0 = blockIdx.y * kGroup + (sub >> 1);
   const int64_t nwarps = ((int64_t)gridDim.x * kKVInt4Threads) >> 5;
-  for (int64_t u = ((int64_t)blockIdx.x * kKVInt4Threads + threadIdx.x) >> 5; u < units; u += nwarps) {
-    const int64_t t = u / groups;
-    const int head0 = (int)(u - t * groups) * kGroup + (sub >> 1);
+  for (int64_t t = ((int64_t)blockIdx.x * kKVInt4Threads + threadIdx.x) >> 5; t < a.T; t += nwarps) {
     const KVSlot slot = kv_int4_slot<PosT>(a, t);
     if (slot.entry == -1 && lane == 0) flag_status(a.status, MAS_STATUS_KV_SLOT_OUT_OF_RANGE);
     const uint8_t* codes = (is_v ? a.kv.v_codes : a.kv.k_codes) + slot.page * a.kv.stride_page +

@@ -637,6 +637,14 @@ int make_alloc_args(AllocArgs* out, const int32_t* delta_lens, int32_t* seq_lens
   return MAS_OK;
 }
 
+// log2 of a power of two, -1 for others.
+int32_t page_shift(int64_t page_size) {
+  if (page_size & (page_size - 1)) return -1;
+  int32_t s = 0;
+  while ((1ll << s) < page_size) ++s;
+  return s;
+}
+
 int make_int4_cache(KVInt4Args* out, const MasInt4KVCache* c, int64_t num_kv_heads, int64_t head_size) {
   if (!c || !c->k_codes || !c->v_codes || !c->pairs || c->num_pages < 0 || c->num_pages > INT32_MAX ||
       c->page_size <= 0 || c->page_size > INT32_MAX || num_kv_heads <= 0 || num_kv_heads > INT32_MAX ||
@@ -662,9 +670,11 @@ int launch_kv_int4_t(const KVInt4RowArgs& a, bool vec, DeviceState* st, void* st
   const auto kernel = READ ? (vec ? read_kv_int4_kernel<T, PosT, D, true> : read_kv_int4_kernel<T, PosT, D, false>)
                            : (vec ? append_kv_int4_kernel<T, PosT, D, true> : append_kv_int4_kernel<T, PosT, D, false>);
   const int64_t group = (int64_t)(256 / D / 2) * kKVInt4Unroll;  // heads a warp
-  const int64_t units = a.T * ceil_div(a.kv.heads, group);
+  const int64_t groups = ceil_div(a.kv.heads, group);
+  if (groups > 65535) return MAS_ERR_UNSUPPORTED_SHAPE;
   const int64_t resident = (int64_t)st->sm_count * resident_ctas((const void*)kernel, kKVInt4Threads, 0);
-  const dim3 grid((unsigned)std::min(ceil_div(units, kKVInt4Threads / 32), resident));
+  const dim3 grid((unsigned)std::min(ceil_div(a.T, kKVInt4Threads / 32), std::max<int64_t>(resident / groups, 1)),
+                  (unsigned)groups);
   return launch(kernel, grid, dim3(kKVInt4Threads), 0, stream, enable_pdl, a);
 }
 
@@ -683,6 +693,7 @@ int run_kv_int4(KVInt4RowArgs a, const MasInt4KVCache* cache, int64_t num_kv_hea
   DeviceState* st = nullptr;
   if ((rc = current_device(&st)) != MAS_OK) return rc;
   if (a.status == nullptr) a.status = st->status;
+  a.page_shift = page_shift(a.kv.page_size);
   const bool vec = aligned(a.k, 16) && aligned(a.v, 16) && a.ksn % 8 == 0 && a.ksh % 8 == 0 && a.vsn % 8 == 0 &&
                    a.vsh % 8 == 0;
   const bool i64 = positions_dtype == MAS_DTYPE_INT64, big = head_size == 128;
@@ -1328,9 +1339,7 @@ int mas_paged_attention_int4(const void* query, void* out, float* lse, const Mas
   a.desc = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + attn_part_bytes(*st, head_size));
   a.scale_log2 = sm_scale * 1.4426950408889634f;
   a.B = (int32_t)batch_size; a.max_blocks = (int32_t)max_blocks; a.group = (int32_t)(num_q_heads / num_kv_heads);
-  a.page_shift = -1;
-  if ((a.kv.page_size & (a.kv.page_size - 1)) == 0)
-    for (a.page_shift = 0; (1ll << a.page_shift) < a.kv.page_size; ++a.page_shift) {}
+  a.page_shift = page_shift(a.kv.page_size);
   a.causal = causal ? 1 : 0;
   a.cta_heads = num_kv_heads % 2 == 0 ? 2 : 1;
   a.q_vec = aligned(query, 16) && q_stride_token % 8 == 0 && q_stride_head % 8 == 0;
