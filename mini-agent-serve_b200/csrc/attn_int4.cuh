@@ -61,7 +61,8 @@ struct AttnInt4Args {
   int32_t page_shift;          // log2(page_size), or -1
   int32_t causal;
   int32_t cta_heads;           // 1 or 2
-  int32_t q_vec;               // rows of queries are 16-byte aligned
+  int32_t q_vec, o_vec;        // rows of queries, of results are 16-byte aligned
+  int32_t split_rows;          // requests with more rows are the prompt kernel's
   uint32_t page16, entry16;    // the codes' strides in units of 16 bytes
   int32_t* status;
 };
@@ -214,7 +215,7 @@ struct AttnRequest {
 };
 
 template <int ROWS>
-__device__ __forceinline__ AttnRequest attn_request(const AttnInt4Args& a, int b, int32_t* status) {
+__device__ __forceinline__ AttnRequest attn_request(const AttnInt4Args& a, int b, int32_t* status, bool few = true) {
   const int unit = kAttnRun * (kAttnWarps / a.cta_heads);
   AttnRequest r;
   int64_t q0 = b, q1 = b + 1;
@@ -233,7 +234,8 @@ __device__ __forceinline__ AttnRequest attn_request(const AttnInt4Args& a, int b
   r.q0 = (int32_t)q0;
   r.qlen = (int32_t)(q1 - q0);
   r.n = (int32_t)n;
-  r.tiles = (int32_t)(((int64_t)r.qlen * a.group + ROWS - 1) / ROWS);
+  const int64_t rows = (int64_t)r.qlen * a.group;
+  r.tiles = few && rows > a.split_rows ? 0 : (int32_t)((rows + ROWS - 1) / ROWS);
   r.units = max(1, (r.n + unit - 1) / unit);
   return r;
 }

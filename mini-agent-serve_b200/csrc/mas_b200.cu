@@ -12,6 +12,7 @@
 #include <mutex>
 
 #include "attn_int4.cuh"
+#include "attn_int4_prompt.cuh"
 #include "common.cuh"
 #include "embed.cuh"
 #include "kv_int4.cuh"
@@ -115,6 +116,8 @@ cudaError_t opt_in_rope_ring() {
 template <typename T>
 cudaError_t opt_in_attn_int4() {
   cudaError_t e;
+  if ((e = opt_in_smem(attn_int4_prompt_kernel<T, 64>, PromptShape<64>::kSmem)) != cudaSuccess) return e;
+  if ((e = opt_in_smem(attn_int4_prompt_kernel<T, 128>, PromptShape<128>::kSmem)) != cudaSuccess) return e;
   if ((e = opt_in_smem(attn_int4_kernel<T, 64, 1>, AttnInt4Shape<64, 1>::kSmem)) != cudaSuccess) return e;
   if ((e = opt_in_smem(attn_int4_kernel<T, 64, 2>, AttnInt4Shape<64, 2>::kSmem)) != cudaSuccess) return e;
   if ((e = opt_in_smem(attn_int4_kernel<T, 64, 4>, AttnInt4Shape<64, 4>::kSmem)) != cudaSuccess) return e;
@@ -746,9 +749,21 @@ int launch_attn_int4(AttnInt4Args a, DeviceState* st, void* stream, int enable_p
 }
 
 template <typename T, int D>
-int run_attn_int4(const AttnInt4Args& a, DeviceState* st, void* stream, int enable_pdl) {
-  // Rows that share a request's kv head, on average: the tile takes them in one go up to 32.
-  const int64_t rows = ceil_div(a.T, a.B) * a.group;
+int run_attn_int4(AttnInt4Args a, DeviceState* st, void* stream, int enable_pdl) {
+  // Rows that share a request's kv head, on average. The lengths are the device's: where some request may have more
+  // than split_rows rows, the prompt kernel is launched for those and this one leaves them out; both may find nothing.
+  int64_t rows = ceil_div(a.T, a.B) * a.group;
+  static const int env_split = env_int("MAS_ATTN_SPLIT_ROWS", kAttnSplitRows);
+  a.split_rows = INT32_MAX;
+  if (a.cum_q != nullptr && a.T * a.group > env_split) {
+    a.split_rows = env_split;
+    const int64_t items = (ceil_div(a.T * a.group, kPromptRows) + a.B) * a.kv.heads;
+    const unsigned grid = (unsigned)std::min<int64_t>(items, st->sm_count);
+    const int rc = launch(attn_int4_prompt_kernel<T, D>, dim3(grid), dim3(kPromptThreads), PromptShape<D>::kSmem, stream,
+                          enable_pdl, a, st->fault);
+    if (rc != MAS_OK) return rc;
+    if (rows > env_split) rows = a.group;  // prompts in the mean: what is left are decode rows
+  }
   if (rows <= 8) return launch_attn_int4<T, D, 1>(a, st, stream, enable_pdl);
   if (rows <= 16) return launch_attn_int4<T, D, 2>(a, st, stream, enable_pdl);
   return launch_attn_int4<T, D, 4>(a, st, stream, enable_pdl);
@@ -1343,6 +1358,7 @@ int mas_paged_attention_int4(const void* query, void* out, float* lse, const Mas
   a.causal = causal ? 1 : 0;
   a.cta_heads = num_kv_heads % 2 == 0 ? 2 : 1;
   a.q_vec = aligned(query, 16) && q_stride_token % 8 == 0 && q_stride_head % 8 == 0;
+  a.o_vec = aligned(out, 16) && out_stride_token % 8 == 0 && out_stride_head % 8 == 0;
   a.page16 = (uint32_t)(a.kv.stride_page >> 4);
   a.entry16 = (uint32_t)(a.kv.stride_entry >> 4);
   a.status = status != nullptr ? status : st->status;

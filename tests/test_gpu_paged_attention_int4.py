@@ -7,6 +7,8 @@ Tolerance, per element, from the kernel's arithmetic (p normalised, n keys):
 - a logit is off by delta = sm_scale 2^-23 (D / 8 + 6) max_t (143 s_t + |m_t|) sum |q|: D / 16 steps of the matrix unit, two
   roundings each, and six more operations, on terms of at most 15 s |q|. It enters as 2 delta (sum p |v| + |o|);
 - the result is rounded: eps_T / 2 |o|.
+Requests with more than 64 rows a kv head take the tensor-core kernel, where u = eps_T / 2 is the rounding of the keys, of the values and of
+the weights: delta = sm_scale max_t sum |q k_t| (u + 2^-23 (D / 8 + 6)), and the weights' part is (2 u + 2^-22 (n / 16 + 32)) sum p |v|.
 """
 from __future__ import annotations
 
@@ -79,6 +81,14 @@ def _bound(q, cache, layout, table, lens, cum, scale, causal, dtype):
             reach = (143 * pr[:seen, :, 0] + pr[:seen, :, 1].abs()).amax(0)  # [h]
             delta = (2.0 ** -23 * (d / 8 + 6) * abs(scale) * reach[:, None] * qi.abs().sum(-1))[..., None]
             o = out[i].view(h, hq // h, d).abs()
+            if (cum[b + 1] - cum[b]) * (hq // h) > 64:
+                u = torch.finfo(dtype).eps / 2
+                terms = torch.einsum("hgd,thd->hgt", qi.abs(), k[:seen].abs()).amax(-1)
+                delta = (abs(scale) * (u + 2.0 ** -23 * (d / 8 + 6)) * terms)[..., None]
+                bound = (2 * u + steps) * size + 2 * delta * (size + o) + u * o
+                tol[i] = bound.reshape(hq, d) + torch.finfo(dtype).tiny
+                ltol[i] = (delta[..., 0] * 1.4427 + 2.0 ** -20 * (1 + lse[i].view(h, -1).abs())).reshape(hq) + steps
+                continue
             bound = 2.0 ** -11 * weights + steps * (sums + minima) + 2 * delta * (size + o) + torch.finfo(dtype).eps / 2 * o
             tol[i] = bound.reshape(hq, d) + torch.finfo(dtype).tiny
             # log2: the logits' error, the sum's and the logarithm's
@@ -152,6 +162,50 @@ def test_page_sizes(cuda, layout, page_size):
 def test_ragged_queries(cuda, dtype, causal, lens, qlens):
     _run(7, lens, qlens, 12, 2, 64, dtype, causal=causal)
     _run(8, lens, qlens, 24, 2, 128, dtype, causal=causal, page_size=5, layout="HND")
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("d,hq,hkv,lens,qlens", [
+    (128, 12, 1, [50], [11]),                     # one step, two tiles of rows
+    (128, 8, 1, [300], [10]),                     # one tile, several steps
+    (64, 12, 2, [129, 128, 127], [30, 128, 7]),
+    (128, 24, 2, [400, 3, 1000], [100, 3, 1]),    # beside short requests, which the other kernel takes
+    (64, 4, 4, [0, 700, 90, 20], [0, 333, 90, 0]),
+    (128, 17, 1, [40], [64]),                     # more queries than tokens
+])
+def test_prompt_rows(cuda, dtype, d, hq, hkv, lens, qlens):
+    _run(61, lens, qlens, hq, hkv, d, dtype)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_prompt_rows_of_odd_pages_and_scales(cuda, causal):
+    _run(62, [333, 70], [150, 70], 6, 2, 128, FP, page_size=5, layout="HND", causal=causal)
+    _run(63, [333, 70], [150, 70], 6, 2, 128, BF, page_size=24, causal=causal, scale=-0.2)
+    _run(64, [333], [150], 6, 2, 64, BF, page_size=1, causal=causal, q_gain=30.0)
+    _run(65, [500], [40], 6, 2, 128, FP, causal=causal, v_scale=1e-4)
+    _run(66, [500], [40], 6, 2, 128, BF, causal=causal, v_scale=1e30)
+
+
+def test_prompt_rows_over_many_items_and_requests(cuda):
+    rng = random.Random(5)
+    lens = [rng.choice([0, 5, 200, 260]) for _ in range(70)]
+    qlens = [min(n, rng.choice([0, 1, 40, 60])) for n in lens]
+    _run(67, lens, qlens, 16, 4, 64, BF)
+
+
+def test_hidden_nan_keys_do_not_reach_earlier_prompt_rows(cuda):
+    lens, qlens = [150], [100]
+    cache, table = _make(68, lens, 2, 128, 16, "NHD")
+    q = torch.randn(100, 8, 128).to(BF).cuda()
+    args = (table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), torch.tensor([0, 100], dtype=torch.int32).cuda())
+    want = mas_b200.paged_attention_int4(q, tuple(t.cuda() for t in cache), *args)
+    for column in (slice(0, 2), slice(2, 4)):  # the keys' pair, the values' pair
+        bad = [t.clone() for t in cache]
+        t = 120  # seen by queries 70 and on
+        bad[2][table[0, t // 16].long(), :, t % 16, column] = math.nan
+        got = mas_b200.paged_attention_int4(q, tuple(t.cuda() for t in bad), *args)
+        assert_bits_equal(got[:70], want[:70], "queries before the NaN")
+        assert got[70:].isnan().all()
 
 
 @pytest.mark.parametrize("dtype", [BF, FP])
