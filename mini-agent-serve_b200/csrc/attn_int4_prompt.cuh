@@ -7,9 +7,9 @@
 // (row, key) then, where it would cost two of the five instructions the softmax spends on one.
 //
 // A CTA takes 256 rows of one kv head (two tiles of 128, the height of an MMA) and walks the keys in steps of 128:
-//   warps 8-11   unpack a step's codes into shared memory: K [key][D] and V [key][D], 128-byte rows of 64 elements, 16-byte
-//                chunks exchanged by the row's last three bits (the 128-byte swizzle), two stages each
-//   warp 12      one thread issues the products: S = Q K^T (both operands from shared memory, both K-major), then
+//   warps 8-15   unpack a step's codes into shared memory, a thread a key: K [key][D] (8-11) and V [key][D] (12-15), 128-byte
+//                rows of 64 elements, 16-byte chunks exchanged by the row's last three bits (the 128-byte swizzle), two stages
+//   warp 16      one thread issues the products: S = Q K^T (both operands from shared memory, both K-major), then
 //                O += P V (P from tensor memory, V from shared memory, MN-major)
 //   warps 0-7    softmax, a thread a row: S from tensor memory, P = 2^(S c - m) back over S as 16-bit pairs; while one tile's
 //                rows are at it the other tile's products run
@@ -25,7 +25,9 @@
 
 namespace mas {
 
-constexpr int kPromptThreads = 416;
+constexpr int kPromptThreads = 544;
+// Registers of the roles; 256 x 128 + 256 x 64 + 32 x 56 stay below the 544 x 96 that the block is launched with.
+constexpr int kPromptSoftmaxRegs = 128, kPromptUnpackRegs = 64, kPromptIssueRegs = 56;
 constexpr int kPromptRows = 256;  // rows of a CTA's item
 constexpr int kPromptKeys = 128;  // keys of a step
 constexpr int kAttnSplitRows = 64;  // requests with more rows a kv head go to this kernel
@@ -89,6 +91,24 @@ __device__ __forceinline__ void tmem_ld32(uint32_t (&r)[32], uint32_t addr) {
         "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(addr));
 }
+// 64 columns of this thread's lane; the wait is part of the statement, so that nothing uses the registers before it.
+__device__ __forceinline__ void tmem_ld64(uint32_t (&r)[64], uint32_t addr) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
+      "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
+      "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]),
+        "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]),
+        "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]),
+        "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]),
+        "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+      : "r"(addr));
+}
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(
@@ -148,9 +168,10 @@ struct ValueUnpack<__half> {
   }
 };
 
-// One key's codes into its row of a 128-row operand. Values that leave T's range are kept at its end.
+// One key's codes into its row of a 128-row operand, each eight elements in the order 0 4 1 5 2 6 3 7 they unpack in
+// (the queries and the results take the same one). Values that leave T's range are kept at its end.
 template <typename T, int D>
-__device__ __forceinline__ void unpack_row(uint32_t base, int row, const uint32_t (&w)[D / 8], uint32_t pair, uint32_t poison) {
+__device__ __forceinline__ void unpack_row(uint32_t base, int row, const uint32_t (&w)[D / 8], uint32_t pair) {
   const ValueUnpack<T> value(pair);
   const float s = __uint_as_float(pair << 16), m = __uint_as_float(pair & 0xffff0000u);
   const bool far = fmaf(15.0f, s, m) > kv_top<T>() || m < -kv_top<T>();
@@ -171,10 +192,8 @@ __device__ __forceinline__ void unpack_row(uint32_t base, int row, const uint32_
         v[i] = Elem<T>::from_f2(f[0], f[1]);
       }
     }
-    const uint32_t a0 = __byte_perm(v[0], v[1], 0x5410) | poison, a1 = __byte_perm(v[2], v[3], 0x5410) | poison;
-    const uint32_t a2 = __byte_perm(v[0], v[1], 0x7632) | poison, a3 = __byte_perm(v[2], v[3], 0x7632) | poison;
     const uint32_t dst = base + (c >> 3) * 16384 + row * 128 + (((c & 7) ^ (row & 7)) << 4);
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(a0), "r"(a1), "r"(a2), "r"(a3) : "memory");
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
   }
 }
 
@@ -258,7 +277,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
     }
     fence_barrier_init();
   }
-  if (warp == 12) {
+  if (warp == 16) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s_tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     tmem_fence_before();
@@ -282,12 +301,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
 
   if (warp < 8) {
     // ---------------- softmax: thread = row ----------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPromptSoftmaxRegs));
     const int tile = warp >> 2, r = tid & 127;
     const uint32_t row_sel = (uint32_t)(warp & 3) << 21;  // this warp's 32 lanes of tensor memory
     const uint32_t s_addr = tmem + row_sel + tile * 128, o_addr = tmem + row_sel + 256 + tile * 128;
     // A negative softmax scale becomes a positive one of negated queries, so that the largest product is the largest logit.
-    const float scale = fabsf(a.scale_log2);
+    const float scale = fmaxf(fabsf(a.scale_log2), 1e-37f);  // not 0, which would make NaNs of hidden columns
     const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
+    // Columns from `left` on are hidden from the row.
+    auto hide = [&](uint32_t (&s)[64], int left) {
+#pragma unroll
+      for (int i = 0; i < 64; ++i) s[i] = i < left ? s[i] : 0xff800000u;
+    };
     uint32_t s_phase = 0, o_phase = 0;
     bool go = true;
     for (int64_t item = blockIdx.x; go && next_item(item); item += gridDim.x) {
@@ -304,6 +329,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
         for (int c = 0; c < D / 8; ++c) {
           Vec16 v = {0, 0, 0, 0};
           if (here) v = a.q_vec ? kv_load8<true>(src + 8 * c) : kv_load8<false>(src + 8 * c);
+          v = Vec16{__byte_perm(v.a, v.c, 0x5410), __byte_perm(v.a, v.c, 0x7632), __byte_perm(v.b, v.d, 0x5410),
+                    __byte_perm(v.b, v.d, 0x7632)};
           const uint32_t dst = base + Sh::kQ + tile * Sh::kTile + (c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4);
           asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.a ^ flip), "r"(v.b ^ flip), "r"(v.c ^ flip),
                        "r"(v.d ^ flip)
@@ -325,13 +352,20 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
         const bool edge = __any_sync(0xffffffffu, left < kPromptKeys);
         // The row's largest logit first: P overwrites S, so nothing may be left to do again.
         float top = -INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < 2; ++c) {
+          uint32_t s[64];
+          tmem_ld64(s, s_addr + c * 64);
+          if (edge) {
+            hide(s, left - c * 64);
+          }
+          float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t s[32];
-          tmem_ld32(s, s_addr + c * 32);
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            top = fmaxf(top, edge && c * 32 + i >= left ? -INFINITY : __uint_as_float(s[i]));
+          for (int i = 0; i < 64; i += 4) {
+            t0 = fmaxf(t0, fmaxf(__uint_as_float(s[i]), __uint_as_float(s[i + 1])));
+            t1 = fmaxf(t1, fmaxf(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3])));
+          }
+          top = fmaxf(top, fmaxf(t0, t1));
         }
         top *= scale;
         const bool up = top > m + 8.0f;
@@ -353,22 +387,19 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
         }
         const float ref = m == -INFINITY ? 0.0f : -m;
         float2 part = make_float2(0.0f, 0.0f);
+#pragma unroll 1
+        for (int c = 0; c < 2; ++c) {
+          uint32_t s[64], p[32];
+          tmem_ld64(s, s_addr + c * 64);
+          if (edge) hide(s, left - c * 64);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t s[32], p[16];
-          tmem_ld32(s, s_addr + c * 32);
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            float2 x = fma2_f32(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), both(scale), both(ref));
-            if (edge) {
-              x.x = c * 32 + i < left ? x.x : -INFINITY;
-              x.y = c * 32 + i + 1 < left ? x.y : -INFINITY;
-            }
+          for (int i = 0; i < 64; i += 2) {
+            const float2 x = fma2_f32(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), both(scale), both(ref));
             const float2 e = make_float2(ex2(x.x), ex2(x.y));
             part = add2_f32(part, e);
             p[i / 2] = Elem<T>::from_f2(e.x, e.y);
           }
-          tmem_st16(s_addr + c * 16, p);  // columns that this thread has read
+          tmem_st32(s_addr + c * 32, p);  // columns that this thread has read
         }
         l += part.x + part.y;
         tmem_wait_st();
@@ -398,7 +429,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
         for (int i = 0; i < 32; i += 8) {
           float f[8];
 #pragma unroll
-          for (int x = 0; x < 8; ++x) f[x] = l != 0.0f ? __uint_as_float(o[i + x]) * inv : 0.0f;
+          for (int x = 0; x < 8; ++x) f[x] = l != 0.0f ? __uint_as_float(o[i + (x < 4 ? 2 * x : 2 * x - 7)]) * inv : 0.0f;
           if (here) {
             if (a.o_vec) kv_store8<true>(dst + c * 32 + i, pack8<T>(f));
             else kv_store8<false>(dst + c * 32 + i, pack8<T>(f));
@@ -410,67 +441,75 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
         a.lse[(int64_t)(it.rq.q0 + tok) * heads * a.group + (int64_t)it.head * a.group + sub] =
             l != 0.0f ? m + __log2f(l) : -INFINITY;
     }
-  } else if (warp < 12) {
-    // ---------------- unpacking: thread = key ----------------
-    const int r = tid - 256;
+  } else if (warp < 16) {
+    // ---------------- unpacking: thread = key; warps 8-11 the keys, 12-15 the values ----------------
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPromptUnpackRegs));
+    const bool values = warp >= 12;
+    const int r = tid & 127;
+    const uint8_t* codes = values ? a.kv.v_codes : a.kv.k_codes;
+    const uint32_t operand = base + (values ? Sh::kV : Sh::kK);
+    const int full = values ? kVFull : kKFull, empty = values ? kVEmpty : kKEmpty;
     constexpr int kVecs = D / 32;  // 16-byte vectors of a row's codes
     uint32_t done = 0;             // steps unpacked so far, over all items
     bool go = true;
     for (int64_t item = blockIdx.x; go && next_item(item); item += gridDim.x) {
       const int32_t* table = a.block_tables + (int64_t)it.b * a.table_stride;
-      uint32_t kw[D / 8], vw[D / 8];
-      uint2 pair;
-      // One step's codes of this thread's key, zeros past the cache's end and on bad pages.
-      auto load = [&](int j) {
+      // The page of this thread's key in step j, -1 past the cache's end and for a bad one.
+      auto find = [&](int j) {
         const int tok = j * kPromptKeys + r;
-        int page = -1;
-        if (j < it.steps && tok < it.rq.n) {
-          page = table[a.page_shift >= 0 ? tok >> a.page_shift : tok / (int)a.kv.page_size];
-          if (page < 0 || page >= a.kv.num_pages) {
-            flag_status(a.status, MAS_STATUS_KV_SLOT_OUT_OF_RANGE);
-            page = -1;
-          }
-        }
+        if (j >= it.steps || tok >= it.rq.n) return -1;
+        const int page = table[a.page_shift >= 0 ? tok >> a.page_shift : tok / (int)a.kv.page_size];
+        if (page >= 0 && page < a.kv.num_pages) return page;
+        if (!values) flag_status(a.status, MAS_STATUS_KV_SLOT_OUT_OF_RANGE);
+        return -1;
+      };
+      // Its codes and pairs there; zeros without a page.
+      auto load = [&](int j, int page, uint32_t (&w)[D / 8], uint2& pair) {
         pair = make_uint2(0, 0);
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) w[i] = 0;
         if (page >= 0) {
+          const int tok = j * kPromptKeys + r;
           const int entry = a.page_shift >= 0 ? tok & ((1 << a.page_shift) - 1) : tok % (int)a.kv.page_size;
           const int64_t off = page * a.kv.stride_page + entry * a.kv.stride_entry + it.head * a.kv.stride_head;
           pair = *reinterpret_cast<const uint2*>(a.kv.pairs + page * a.kv.pair_stride_page +
                                                  ((int64_t)it.head * a.kv.page_size + entry) * 4);
 #pragma unroll
           for (int i = 0; i < kVecs; ++i) {
-            const Vec16 k = ld_ro(a.kv.k_codes + off + 16 * i), v = ld_ro(a.kv.v_codes + off + 16 * i);
-            kw[4 * i] = k.a; kw[4 * i + 1] = k.b; kw[4 * i + 2] = k.c; kw[4 * i + 3] = k.d;
-            vw[4 * i] = v.a; vw[4 * i + 1] = v.b; vw[4 * i + 2] = v.c; vw[4 * i + 3] = v.d;
+            const Vec16 x = ld_ro(codes + off + 16 * i);
+            w[4 * i] = x.a; w[4 * i + 1] = x.b; w[4 * i + 2] = x.c; w[4 * i + 3] = x.d;
           }
-        } else {
-#pragma unroll
-          for (int i = 0; i < D / 8; ++i) kw[i] = vw[i] = 0;
         }
       };
-      load(0);
+      // The codes of the next step and the page of the one after it are on their way while a step is unpacked.
+      uint32_t w[D / 8];
+      uint2 pair;
+      load(0, find(0), w, pair);
+      int page = find(1);
       for (int j = 0; j < it.steps; ++j, ++done) {
         const int stage = done & 1;
-        const uint32_t free_parity = ((done >> 1) & 1) ^ 1;  // the first use of a stage finds it free
+        uint32_t w_next[D / 8];
+        uint2 pair_next;
+        load(j + 1, page, w_next, pair_next);
+        page = find(j + 2);
+        // The first use of a stage finds it free.
+        go = __all_sync(0xffffffffu, wait(empty + stage, ((done >> 1) & 1) ^ 1));
+        if (!go) break;
         // A value row that is not finite may be hidden from some rows, whose zero weights would not hide it: it is
         // replaced by zeros and its key by NaNs, which reach exactly the rows that see it.
         const float vf = fmaf(__uint_as_float(pair.y << 16), 0.0f, __uint_as_float(pair.y & 0xffff0000u) * 0.0f);
-        const bool bad = vf != 0.0f;
-        go = __all_sync(0xffffffffu, wait(kKEmpty + stage, free_parity));
-        if (!go) break;
-        unpack_row<T, D>(base + Sh::kK + stage * Sh::kTile, r, kw, pair.x, bad ? 0x7fff7fffu : 0u);
+        const uint32_t mine = values ? (vf != 0.0f || vf != vf ? 0u : pair.y) : (vf != 0.0f || vf != vf ? 0x7fc07fc0u : pair.x);
+        unpack_row<T, D>(operand + stage * Sh::kTile, r, w, mine);
         fence_proxy_async_smem();
-        mbar_arrive(&bars[kKFull + stage]);
-        go = __all_sync(0xffffffffu, wait(kVEmpty + stage, free_parity));
-        if (!go) break;
-        unpack_row<T, D>(base + Sh::kV + stage * Sh::kTile, r, vw, bad ? 0u : pair.y, 0u);
-        fence_proxy_async_smem();
-        mbar_arrive(&bars[kVFull + stage]);
-        load(j + 1);
+        mbar_arrive(&bars[full + stage]);
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) w[i] = w_next[i];
+        pair = pair_next;
       }
     }
   } else {
     // ---------------- products: lane 0 issues, the others walk along ----------------
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPromptIssueRegs));
     constexpr uint32_t kIdescS = umma_idesc<T>(128, kPromptKeys, false), kIdescO = umma_idesc<T>(128, D, true);
     uint32_t done = 0, q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
     bool go = true;
@@ -536,7 +575,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
   __syncwarp();
   tmem_fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 16) {
     tmem_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
   }
