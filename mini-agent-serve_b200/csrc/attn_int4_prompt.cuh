@@ -2,21 +2,27 @@
 // fifth-generation tensor cores (sm_100a).
 //
 // The same mathematics as attn_int4.cuh, with another bound: a request's rows (tokens x group) outnumber what a key
-// brings in, so the products decide, 4 * D flops a row and key, and each key is unpacked once for 256 rows. Keys and values
-// enter the products as c * s + m rounded once to the queries' type, like a cache held in that type: the pair costs nothing per
-// (row, key) then, where it would cost two of the five instructions the softmax spends on one.
+// brings in, so the products decide, 4 * D flops a row and key, and each key is unpacked once for 256 rows. Here, too, the products
+// run on bare codes (c - 8 in fp16, exact) and the pairs enter in fp32, between them:
+//   y = S' ks + (sum q) kb,  p = 2^(y - M),  l += p,  r += p (mv + 8 sv),  w = fp16(p sv),  O += w (cv - 8),  o = (O + r) / l
+// (ks, kb the key's scale and minimum + 8 scales, times the softmax scale and log2 e). Keys and values rounded to bf16 on the
+// way in, which needs two of these eight instructions less a (row, key), took 924 us at the case below, but were 0.0051 of the
+// result off where this is 0.0018. M is one reference for all: the row's largest log2 of a weight p sv, moved when one passes it by 8.
 //
 // A CTA takes 256 rows of one kv head (two tiles of 128, the height of an MMA) and walks the keys in steps of 128:
 //   warps 8-15   unpack a step's codes into shared memory, a thread a key: K [key][D] (8-11) and V [key][D] (12-15), 128-byte
 //                rows of 64 elements, 16-byte chunks exchanged by the row's last three bits (the 128-byte swizzle), two stages
-//   warp 16      one thread issues the products: S = Q K^T (both operands from shared memory, both K-major), then
-//                O += P V (P from tensor memory, V from shared memory, MN-major)
-//   warps 0-7    softmax, a thread a row: S from tensor memory, P = 2^(S c - m) back over S as 16-bit pairs; while one tile's
-//                rows are at it the other tile's products run
-// Tensor memory: S0 S1 O0 O1, 128 fp32 columns each, all 512. The reference m moves only when a logit passes it by 8, and
-// then the thread rescales its row of O, which no product touches between the two barriers it stands between.
+//   warps 0-7    softmax, a thread a row, 64 keys of a step at a time: S from tensor memory, the logits y and their maximum, the
+//                weights, over the first half of S as 16-bit pairs; while one tile's rows are at it the other tile's products
+//                run. A thread of each tile's first warp issues them: S = Q K^T (both operands from shared
+//                memory, K-major), then O += P V (P from tensor memory, V from shared memory, MN-major)
+// Tensor memory: S0 S1 O0 O1, 128 fp32 columns each, all 512. When M moves, the thread rescales its row of O, which no
+// product touches between the two barriers it stands between. The keys' and values' factors travel through shared memory, four
+// steps deep: a step's are overwritten four steps on, when the products of two steps on, which followed its rows' softmax, are done.
 // Every wait is bounded; one that runs out sets the fault word and all roles leave.
 #pragma once
+
+#include <math_constants.h>
 
 #include <type_traits>
 
@@ -25,9 +31,10 @@
 
 namespace mas {
 
-constexpr int kPromptThreads = 544;
-// Registers of the roles; 256 x 128 + 256 x 64 + 32 x 56 stay below the 544 x 96 that the block is launched with.
-constexpr int kPromptSoftmaxRegs = 128, kPromptUnpackRegs = 64, kPromptIssueRegs = 56;
+constexpr int kPromptThreads = 512;
+// Registers of the roles: 8 warps x 168 + 8 warps x 88 = 16 warps x 128, what the block is launched with (on every quarter of
+// the SM, too).
+constexpr int kPromptSoftmaxRegs = 168, kPromptUnpackRegs = 88;
 constexpr int kPromptRows = 256;  // rows of a CTA's item
 constexpr int kPromptKeys = 128;  // keys of a step
 constexpr int kAttnSplitRows = 64;  // requests with more rows a kv head go to this kernel
@@ -38,11 +45,18 @@ struct PromptShape {
   static constexpr int kQ = 0;               // two tiles
   static constexpr int kK = 2 * kTile;       // two stages
   static constexpr int kV = 4 * kTile;       // two stages
-  static constexpr int kBars = 6 * kTile;
+  static constexpr int kKeyFactors = 6 * kTile;              // [4][64 pairs of keys] {ks, ks, kb, kb}
+  static constexpr int kValueFactors = kKeyFactors + 4096;   // [4][64 pairs of keys] {sv, sv, mv + 8 sv, mv + 8 sv}
+  static constexpr int kLogs = kValueFactors + 4096;         // [4][128] log2 sv
+  static constexpr int kSpread = kLogs + 2048;               // [4][4 warps] {largest, smallest log2 sv}
+  static constexpr int kBars = kSpread + 128;
   static constexpr int kSmem = kBars + 256 + 1024;  // the operands are aligned to 1024 bytes by hand
 };
 
-enum PromptBar { kKFull = 0, kKEmpty = 2, kVFull = 4, kVEmpty = 6, kSFull = 8, kPFull = 10, kQFull = 12, kOFull = 14, kPromptBars = 16 };
+enum PromptBar { kKFull = 0, kKEmpty = 2, kVFull = 4, kVEmpty = 6, kSFull = 8, kPFull = 10, kQFull = 12, kOFull = 14, kKeyFac = 16, kValueFac = 20,
+                 kDrain = 24, kPromptBars = 26 };
+// Up to this spread of the values' scales (log2) in a step, the largest stands for all in the choice of M.
+constexpr float kPromptSpread = 10.0f;
 
 // Shared-memory operand descriptor, 128-byte swizzle. K-major: rows of 128 bytes, groups of eight rows `sbo` bytes apart.
 // MN-major: `lbo` bytes between blocks of 64 elements of the long axis, `sbo` between groups of eight of the other.
@@ -50,12 +64,9 @@ __device__ __forceinline__ uint64_t umma_desc(uint32_t addr, uint32_t lbo, uint3
   return (uint64_t)((addr & 0x3ffffu) >> 4) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(sbo >> 4) << 32) | (1ull << 46) |
          (2ull << 61);
 }
-// Instruction descriptor of kind::f16: fp32 accumulators, both operands of one 16-bit type.
-template <typename T>
+// Instruction descriptor of kind::f16: fp32 accumulators, both operands fp16.
 __device__ __forceinline__ constexpr uint32_t umma_idesc(int m, int n, bool b_mn_major) {
-  const uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-  return (1u << 4) | (type << 7) | (type << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
-         ((uint32_t)(m >> 4) << 24);
+  return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 __device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
   asm volatile(
@@ -109,14 +120,6 @@ __device__ __forceinline__ void tmem_ld64(uint32_t (&r)[64], uint32_t addr) {
         "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
       : "r"(addr));
 }
-__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(
-          addr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
-}
 __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, "
@@ -135,62 +138,21 @@ __device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t m
   return r;
 }
 
-// The codes of one word (elements 8i .. 8i + 7, packed 0-4, 1-5, 2-6, 3-7) as values c * s + m in T, one rounding each.
-template <typename T>
-struct ValueUnpack;
-template <>
-struct ValueUnpack<__nv_bfloat16> {
-  __nv_bfloat162 s, m;
-  __device__ __forceinline__ ValueUnpack(uint32_t pair) {
-    const uint32_t ss = __byte_perm(pair, pair, 0x1010), mm = __byte_perm(pair, pair, 0x3232);
-    s = *reinterpret_cast<const __nv_bfloat162*>(&ss);
-    m = *reinterpret_cast<const __nv_bfloat162*>(&mm);
-  }
-  __device__ __forceinline__ uint32_t operator()(uint32_t w, int i) const {
-    uint32_t u = and_or(w >> (4 * i), 0x000f000fu, 0x43004300u);  // 128 + c
-    const __nv_bfloat162 c = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&u), __floats2bfloat162_rn(128.0f, 128.0f));
-    const __nv_bfloat162 v = __hfma2(c, s, m);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  }
-};
-template <>
-struct ValueUnpack<__half> {
-  __half2 s, m;
-  __device__ __forceinline__ ValueUnpack(uint32_t pair) {
-    s = __float2half2_rn(__uint_as_float(pair << 16));
-    m = __float2half2_rn(__uint_as_float(pair & 0xffff0000u));
-  }
-  __device__ __forceinline__ uint32_t operator()(uint32_t w, int i) const {
-    uint32_t u = and_or(w >> (4 * i), 0x000f000fu, 0x64006400u);  // 1024 + c
-    const __half2 c = __hsub2(*reinterpret_cast<__half2*>(&u), __float2half2_rn(1024.0f));
-    const __half2 v = __hfma2(c, s, m);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  }
-};
-
-// One key's codes into its row of a 128-row operand, each eight elements in the order 0 4 1 5 2 6 3 7 they unpack in
-// (the queries and the results take the same one). Values that leave T's range are kept at its end.
-template <typename T, int D>
-__device__ __forceinline__ void unpack_row(uint32_t base, int row, const uint32_t (&w)[D / 8], uint32_t pair) {
-  const ValueUnpack<T> value(pair);
-  const float s = __uint_as_float(pair << 16), m = __uint_as_float(pair & 0xffff0000u);
-  const bool far = fmaf(15.0f, s, m) > kv_top<T>() || m < -kv_top<T>();
+// One key's codes into its row of a 128-row operand as fp16 c - 8, each eight elements in the order 0 4 1 5 2 6 3 7 they
+// unpack in (the queries and the results take the same one): 1024 + c and 1024 + 16 c are exact, and so is what follows.
+template <int D>
+__device__ __forceinline__ void unpack_row(uint32_t base, int row, const uint32_t (&w)[D / 8]) {
+  const __half2 off = __float2half2_rn(1032.0f), sixteenth = __float2half2_rn(0.0625f), off16 = __float2half2_rn(-72.0f);
 #pragma unroll
   for (int c = 0; c < D / 8; ++c) {
     uint32_t v[4];  // pairs (0, 4), (1, 5), (2, 6), (3, 7)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = value(w[c], i);
-    if (far) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float f[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          f[h] = fmaf((float)((w[c] >> (4 * (i + 4 * h))) & 15u), s, m);
-          f[h] = fminf(fmaxf(f[h], -kv_top<T>()), kv_top<T>());
-        }
-        v[i] = Elem<T>::from_f2(f[0], f[1]);
-      }
+    for (int i = 0; i < 2; ++i) {
+      uint32_t lo = and_or(w[c] >> (8 * i), 0x000f000fu, 0x64006400u), hi = and_or(w[c] >> (8 * i), 0x00f000f0u, 0x64006400u);
+      const __half2 x = __hsub2(*reinterpret_cast<__half2*>(&lo), off);
+      const __half2 y = __hfma2(*reinterpret_cast<__half2*>(&hi), sixteenth, off16);
+      v[2 * i] = *reinterpret_cast<const uint32_t*>(&x);
+      v[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&y);
     }
     const uint32_t dst = base + (c >> 3) * 16384 + row * 128 + (((c & 7) ^ (row & 7)) << 4);
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
@@ -211,7 +173,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
   __shared__ volatile int s_stop;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(raw + (base - smem_u32(raw)) + Sh::kBars);
+  uint8_t* shared = raw + (base - smem_u32(raw));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(shared + Sh::kBars);
   pdl_wait();
   // Items in order: requests, heads, row blocks. Each warp walks them for itself, 32 requests at a time (a lane each);
   // all find the same ones.
@@ -267,17 +230,22 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
     s_stop = 0;
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars[kKFull + i], 128);
-      mbar_init(&bars[kKEmpty + i], 1);
+      mbar_init(&bars[kKEmpty + i], 2);  // each tile's products, or one tile's twice
       mbar_init(&bars[kVFull + i], 128);
-      mbar_init(&bars[kVEmpty + i], 1);
+      mbar_init(&bars[kVEmpty + i], 2);
       mbar_init(&bars[kSFull + i], 1);
       mbar_init(&bars[kPFull + i], 128);
       mbar_init(&bars[kQFull + i], 128);
       mbar_init(&bars[kOFull + i], 1);
+      mbar_init(&bars[kDrain + i], 1);
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&bars[kKeyFac + i], 128);
+      mbar_init(&bars[kValueFac + i], 128);
     }
     fence_barrier_init();
   }
-  if (warp == 16) {
+  if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s_tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     tmem_fence_before();
@@ -305,43 +273,100 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
     const int tile = warp >> 2, r = tid & 127;
     const uint32_t row_sel = (uint32_t)(warp & 3) << 21;  // this warp's 32 lanes of tensor memory
     const uint32_t s_addr = tmem + row_sel + tile * 128, o_addr = tmem + row_sel + 256 + tile * 128;
-    // A negative softmax scale becomes a positive one of negated queries, so that the largest product is the largest logit.
-    const float scale = fmaxf(fabsf(a.scale_log2), 1e-37f);  // not 0, which would make NaNs of hidden columns
-    const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
     // Columns from `left` on are hidden from the row.
     auto hide = [&](uint32_t (&s)[64], int left) {
 #pragma unroll
       for (int i = 0; i < 64; ++i) s[i] = i < left ? s[i] : 0xff800000u;
     };
-    uint32_t s_phase = 0, o_phase = 0;
+    // Products, by one thread a tile. Step d (of all items) uses stage d & 1.
+    constexpr uint32_t kIdescS = umma_idesc(128, kPromptKeys, false), kIdescO = umma_idesc(128, D, true);
+    const bool issuer = lane == 0 && (warp & 3) == 0;
+    auto release = [&](int bar) {  // of a stage: with one tile at work its products stand for the other's, too
+      umma_commit(&bars[bar]);
+      if (it.rows <= 128) umma_commit(&bars[bar]);
+    };
+    auto issue_scores = [&](uint32_t d) {
+      const int stage = d & 1;
+      if (!wait(kKFull + stage, (d >> 1) & 1)) return;
+      tmem_fence_after();
+      const uint32_t q = base + Sh::kQ + tile * Sh::kTile, k = base + Sh::kK + stage * Sh::kTile;
+#pragma unroll
+      for (int x = 0; x < D / 16; ++x) {
+        const uint32_t off = (x >> 2) * 16384 + (x & 3) * 32;  // 16 elements of D
+        umma_ss(tmem + tile * 128, umma_desc(q + off, 16, 1024), umma_desc(k + off, 16, 1024), kIdescS, x > 0);
+      }
+      umma_commit(&bars[kSFull + tile]);
+      release(kKEmpty + stage);
+    };
+    auto issue_values = [&](uint32_t d, bool accumulate) {
+      const int stage = d & 1;
+      if (!wait(kVFull + stage, (d >> 1) & 1)) return;
+      tmem_fence_after();
+#pragma unroll
+      for (int x = 0; x < kPromptKeys / 16; ++x)
+        umma_ts(tmem + 256 + tile * 128, tmem + tile * 128 + x * 8,
+                umma_desc(base + Sh::kV + stage * Sh::kTile + x * 2048, 16384, 1024), kIdescO, accumulate || x > 0);
+      release(kVEmpty + stage);
+    };
+    uint32_t s_phase = 0, o_phase = 0, p_phase = 0, q_phase = 0;
+    uint32_t done = 0;  // steps so far, over all items, this tile's rows at work or not
     bool go = true;
     for (int64_t item = blockIdx.x; go && next_item(item); item += gridDim.x) {
-      if (tile * 128 >= it.rows) continue;
+      if (tile * 128 >= it.rows) {
+        done += it.steps;
+        continue;
+      }
       const int row = it.row0 + tile * 128 + r;
       const bool here = tile * 128 + r < it.rows;
       const int tok = (it.row0 + min(tile * 128 + r, it.rows - 1)) / a.group;
       const int sub = row - tok * a.group;
       const int lim = a.causal ? min(it.rq.n, max(0, it.rq.n - it.rq.qlen + tok + 1)) : it.rq.n;
+      float qsum = 0.0f, unscale = 1.0f;
       if (it.steps > 0) {
+        // The row as fp16, a bf16 one scaled by a power of two to a largest element of 2^11 to 2^12 (as in attn_int4.cuh).
         const uint16_t* src = static_cast<const uint16_t*>(a.q) + (int64_t)(it.rq.q0 + tok) * a.qsn +
                               ((int64_t)it.head * a.group + (here ? sub : 0)) * a.qsh;
+        float scale = 1.0f;
+        if (std::is_same<T, __nv_bfloat16>::value) {
+          uint32_t most = 0;
+#pragma unroll 4
+          for (int c = 0; c < D / 8; ++c) {
+            float f[8];
+            unpack8<T>(a.q_vec ? kv_load8<true>(src + 8 * c) : kv_load8<false>(src + 8 * c), f);
 #pragma unroll
+            for (int x = 0; x < 8; ++x) most = max(most, __float_as_uint(fabsf(f[x])));
+          }
+          const uint32_t exponent = min(max(most >> 23, 12u), 254u);
+          scale = __uint_as_float((265u - exponent) << 23);
+          unscale = __uint_as_float((exponent - 11u) << 23);
+        }
+#pragma unroll 4
         for (int c = 0; c < D / 8; ++c) {
-          Vec16 v = {0, 0, 0, 0};
-          if (here) v = a.q_vec ? kv_load8<true>(src + 8 * c) : kv_load8<false>(src + 8 * c);
-          v = Vec16{__byte_perm(v.a, v.c, 0x5410), __byte_perm(v.a, v.c, 0x7632), __byte_perm(v.b, v.d, 0x5410),
-                    __byte_perm(v.b, v.d, 0x7632)};
+          float f[8];
+          unpack8<T>(a.q_vec ? kv_load8<true>(src + 8 * c) : kv_load8<false>(src + 8 * c), f);
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            f[x] = here ? f[x] * scale : 0.0f;
+            qsum += f[x];
+          }
           const uint32_t dst = base + Sh::kQ + tile * Sh::kTile + (c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.a ^ flip), "r"(v.b ^ flip), "r"(v.c ^ flip),
-                       "r"(v.d ^ flip)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(Elem<__half>::from_f2(f[0], f[4])),
+                       "r"(Elem<__half>::from_f2(f[1], f[5])), "r"(Elem<__half>::from_f2(f[2], f[6])),
+                       "r"(Elem<__half>::from_f2(f[3], f[7]))
                        : "memory");
         }
         fence_proxy_async_smem();
         mbar_arrive(&bars[kQFull + tile]);
+        if (issuer && wait(kQFull + tile, q_phase)) issue_scores(done);
+        __syncwarp();
+        q_phase ^= 1;
       }
       float m = -INFINITY, l = 0.0f;
-      for (int j = 0; go && j < it.steps; ++j) {
-        go = wait(kSFull + tile, s_phase);
+      float2 r2 = both(0.0f);
+      for (int j = 0; go && j < it.steps; ++j, ++done) {
+        const int buf = done & 3;
+        const uint32_t parity = (done >> 2) & 1;
+        go = wait(kSFull + tile, s_phase) && wait(kKeyFac + buf, parity) && wait(kValueFac + buf, parity);
         s_phase ^= 1;
         if (!__all_sync(0xffffffffu, go)) {
           go = false;
@@ -350,61 +375,106 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
         tmem_fence_after();
         const int left = lim - j * kPromptKeys;  // keys of this step that the row sees
         const bool edge = __any_sync(0xffffffffu, left < kPromptKeys);
-        // The row's largest logit first: P overwrites S, so nothing may be left to do again.
-        float top = -INFINITY;
+        const uint32_t kf = base + Sh::kKeyFactors + buf * 1024, vf = base + Sh::kValueFactors + buf * 1024;
+        float lv_max = -INFINITY, lv_min = INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 x = lds_float2(base + Sh::kSpread + buf * 32 + i * 8);
+          lv_max = fmaxf(lv_max, x.x);
+          lv_min = fminf(lv_min, x.y);
+        }
+        const bool alike = lv_max - lv_min <= kPromptSpread;
+        // 64 keys at a time: logits, the reference, weights.
 #pragma unroll 1
         for (int c = 0; c < 2; ++c) {
           uint32_t s[64];
           tmem_ld64(s, s_addr + c * 64);
-          if (edge) {
-            hide(s, left - c * 64);
+#pragma unroll
+          for (int i = 0; i < 64; i += 2) {
+            const uint4 f = lds128(kf + (c * 64 + i) * 8);
+            const float2 y = fma2_f32(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])),
+                                      make_float2(__uint_as_float(f.x), __uint_as_float(f.y)),
+                                      mul2_f32(both(qsum), make_float2(__uint_as_float(f.z), __uint_as_float(f.w))));
+            s[i] = __float_as_uint(y.x);
+            s[i + 1] = __float_as_uint(y.y);
           }
+          if (edge) hide(s, left - c * 64);
           float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
           for (int i = 0; i < 64; i += 4) {
             t0 = fmaxf(t0, fmaxf(__uint_as_float(s[i]), __uint_as_float(s[i + 1])));
             t1 = fmaxf(t1, fmaxf(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3])));
           }
-          top = fmaxf(top, fmaxf(t0, t1));
-        }
-        top *= scale;
-        const bool up = top > m + 8.0f;
-        if (__any_sync(0xffffffffu, up)) {
-          const float was = m;
-          m = up ? top : m;
-          const float factor = was == m || was == -INFINITY ? 1.0f : ex2(was - m);  // before its first key the row of O is zeros
-          if (j > 0) {
-#pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t o[32];
-              tmem_ld32(o, o_addr + c * 32);
+          const float top = fmaxf(t0, t1) * unscale;
+          // The largest weight's log2: the largest logit and the largest scale where the scales are alike, each weight's
+          // own where they are not (a hidden key's scale must not set the reference of rows that do not see it).
+          float cand = top + lv_max;
+          if (!alike) {
+            cand = -INFINITY;
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
-              tmem_st32(o_addr + c * 32, o);
+            for (int i = 0; i < 64; i += 2) {
+              const float2 lv = lds_float2(base + Sh::kLogs + buf * 512 + (c * 64 + i) * 4);
+              cand = fmaxf(cand, fmaxf(fmaf(__uint_as_float(s[i]), unscale, lv.x), fmaf(__uint_as_float(s[i + 1]), unscale, lv.y)));
             }
           }
-          l *= factor;
-        }
-        const float ref = m == -INFINITY ? 0.0f : -m;
-        float2 part = make_float2(0.0f, 0.0f);
+          // Values of scale 0 (or next to it) weigh nothing, but p is to stay finite. (Scales past 2^100 would cost l small p's.)
+          cand = fmaxf(cand, top - 100.0f);
+          const bool up = cand > m + 8.0f;
+          if (__any_sync(0xffffffffu, up)) {
+            const float was = m;
+            m = up ? cand : m;
+            const float factor = was == m || was == -INFINITY ? 1.0f : ex2(was - m);  // before its first key the row of O is zeros
+            if (j > 0) {
 #pragma unroll 1
-        for (int c = 0; c < 2; ++c) {
-          uint32_t s[64], p[32];
-          tmem_ld64(s, s_addr + c * 64);
-          if (edge) hide(s, left - c * 64);
+              for (int d = 0; d < D / 32; ++d) {
+                uint32_t o[32];
+                tmem_ld32(o, o_addr + d * 32);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
+                tmem_st32(o_addr + d * 32, o);
+              }
+            }
+            if (c > 0) {  // the first half's weights are relative to the old reference
+              uint32_t w[32];
+              tmem_ld32(w, s_addr);
+              const __half2 by = __float2half2_rn(factor);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                const __half2 x = __hmul2(*reinterpret_cast<__half2*>(&w[i]), by);
+                w[i] = *reinterpret_cast<const uint32_t*>(&x);
+              }
+              tmem_st32(s_addr, w);
+            }
+            l *= factor;
+            r2.x *= factor;
+            r2.y *= factor;
+          }
+          const float ref = m == -INFINITY ? 0.0f : -m;
+          float2 part = both(0.0f);
+          uint32_t w[32];
 #pragma unroll
           for (int i = 0; i < 64; i += 2) {
-            const float2 x = fma2_f32(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), both(scale), both(ref));
-            const float2 e = make_float2(ex2(x.x), ex2(x.y));
-            part = add2_f32(part, e);
-            p[i / 2] = Elem<T>::from_f2(e.x, e.y);
+            const uint4 f = lds128(vf + (c * 64 + i) * 8);
+            const float2 x = fma2_f32(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), both(unscale), both(ref));
+            const float2 p = make_float2(ex2(x.x), ex2(x.y));
+            part = add2_f32(part, p);
+            r2 = fma2_f32(p, make_float2(__uint_as_float(f.z), __uint_as_float(f.w)), r2);
+            const float2 v = mul2_f32(p, make_float2(__uint_as_float(f.x), __uint_as_float(f.y)));
+            w[i / 2] = Elem<__half>::from_f2(v.x, v.y);
           }
-          tmem_st32(s_addr + c * 32, p);  // columns that this thread has read
+          tmem_st32(s_addr + c * 32, w);  // columns that this thread has read
+          l += part.x + part.y;
         }
-        l += part.x + part.y;
         tmem_wait_st();
         tmem_fence_before();
         mbar_arrive(&bars[kPFull + tile]);
+        if (issuer && wait(kPFull + tile, p_phase)) {
+          issue_values(done, j > 0);
+          if (j + 1 < it.steps) issue_scores(done + 1);
+          else umma_commit(&bars[kOFull + tile]);
+        }
+        __syncwarp();
+        p_phase ^= 1;
       }
       if (!go) break;
       if (it.steps > 0) {
@@ -416,7 +486,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
         }
         tmem_fence_after();
       }
-      const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+      const float inv = l != 0.0f ? 1.0f / l : 0.0f, rest = r2.x + r2.y;
       uint16_t* dst = static_cast<uint16_t*>(a.out) + (int64_t)(it.rq.q0 + tok) * a.osn +
                       ((int64_t)it.head * a.group + sub) * a.osh;
 #pragma unroll 1
@@ -429,7 +499,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
         for (int i = 0; i < 32; i += 8) {
           float f[8];
 #pragma unroll
-          for (int x = 0; x < 8; ++x) f[x] = l != 0.0f ? __uint_as_float(o[i + (x < 4 ? 2 * x : 2 * x - 7)]) * inv : 0.0f;
+          for (int x = 0; x < 8; ++x) f[x] = l != 0.0f ? (__uint_as_float(o[i + (x < 4 ? 2 * x : 2 * x - 7)]) + rest) * inv : 0.0f;
           if (here) {
             if (a.o_vec) kv_store8<true>(dst + c * 32 + i, pack8<T>(f));
             else kv_store8<false>(dst + c * 32 + i, pack8<T>(f));
@@ -441,7 +511,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
         a.lse[(int64_t)(it.rq.q0 + tok) * heads * a.group + (int64_t)it.head * a.group + sub] =
             l != 0.0f ? m + __log2f(l) : -INFINITY;
     }
-  } else if (warp < 16) {
+    if (!go && issuer) {
+      // Products may be in flight over shared and tensor memory: let them end (bounded) before anything is freed.
+      umma_commit(&bars[kDrain + tile]);
+      (void)mbar_wait_bounded(&bars[kDrain + tile], 0, kWaitLimitNs / 4);
+    }
+  } else {
     // ---------------- unpacking: thread = key; warps 8-11 the keys, 12-15 the values ----------------
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPromptUnpackRegs));
     const bool values = warp >= 12;
@@ -495,87 +570,48 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
         // The first use of a stage finds it free.
         go = __all_sync(0xffffffffu, wait(empty + stage, ((done >> 1) & 1) ^ 1));
         if (!go) break;
-        // A value row that is not finite may be hidden from some rows, whose zero weights would not hide it: it is
-        // replaced by zeros and its key by NaNs, which reach exactly the rows that see it.
-        const float vf = fmaf(__uint_as_float(pair.y << 16), 0.0f, __uint_as_float(pair.y & 0xffff0000u) * 0.0f);
-        const uint32_t mine = values ? (vf != 0.0f || vf != vf ? 0u : pair.y) : (vf != 0.0f || vf != vf ? 0x7fc07fc0u : pair.x);
-        unpack_row<T, D>(operand + stage * Sh::kTile, r, w, mine);
+        unpack_row<D>(operand + stage * Sh::kTile, r, w);
         fence_proxy_async_smem();
         mbar_arrive(&bars[full + stage]);
+        // A value row that is not finite may be hidden from some rows, whose zero weights would not hide it: its factors
+        // are replaced by zeros and its key's by NaNs, which reach exactly the rows that see it.
+        const float sv = __uint_as_float(pair.y << 16), mv = __uint_as_float(pair.y & 0xffff0000u);
+        const bool bad = !(sv * 0.0f + mv * 0.0f == 0.0f);
+        const int buf = done & 3;
+        float x, y;
+        if (values) {
+          x = bad ? 0.0f : sv;
+          y = bad ? 0.0f : fmaf(8.0f, sv, mv);
+          const float lv = __log2f(x);
+          const bool counts = !bad && j * kPromptKeys + r < it.rq.n;
+          *reinterpret_cast<float*>(shared + Sh::kLogs + buf * 512 + r * 4) = lv;
+          float hi = counts ? lv : -INFINITY, lo = counts ? lv : INFINITY;
+#pragma unroll
+          for (int z = 16; z > 0; z >>= 1) {
+            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, z));
+            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, z));
+          }
+          if (lane == 0) *reinterpret_cast<float2*>(shared + Sh::kSpread + buf * 32 + (warp & 3) * 8) = make_float2(hi, lo);
+          __syncwarp();
+        } else {
+          const float sk = __uint_as_float(pair.x << 16), mk = __uint_as_float(pair.x & 0xffff0000u);
+          x = bad ? CUDART_NAN_F : sk * a.scale_log2;
+          y = bad ? CUDART_NAN_F : fmaf(8.0f, sk, mk) * a.scale_log2;
+        }
+        float* fac = reinterpret_cast<float*>(shared + (values ? Sh::kValueFactors : Sh::kKeyFactors) + buf * 1024 + (r >> 1) * 16);
+        fac[r & 1] = x;
+        fac[2 + (r & 1)] = y;
+        mbar_arrive(&bars[(values ? kValueFac : kKeyFac) + buf]);
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) w[i] = w_next[i];
         pair = pair_next;
       }
     }
-  } else {
-    // ---------------- products: lane 0 issues, the others walk along ----------------
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPromptIssueRegs));
-    constexpr uint32_t kIdescS = umma_idesc<T>(128, kPromptKeys, false), kIdescO = umma_idesc<T>(128, D, true);
-    uint32_t done = 0, q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
-    bool go = true;
-    auto scores = [&](int tile, int stage) {
-      const uint32_t q = base + Sh::kQ + tile * Sh::kTile, k = base + Sh::kK + stage * Sh::kTile;
-#pragma unroll
-      for (int x = 0; x < D / 16; ++x) {
-        const uint32_t off = (x >> 2) * 16384 + (x & 3) * 32;  // 16 elements of D
-        umma_ss(tmem + tile * 128, umma_desc(q + off, 16, 1024), umma_desc(k + off, 16, 1024), kIdescS, x > 0);
-      }
-      umma_commit(&bars[kSFull + tile]);
-    };
-    auto run_item = [&] {
-      bool ok = true;
-      const int tiles = it.rows > 128 ? 2 : 1;
-      ok = wait(kKFull + (done & 1), (done >> 1) & 1);
-      for (int tile = 0; ok && tile < tiles; ++tile) {
-        ok = wait(kQFull + tile, q_phase[tile]);
-        q_phase[tile] ^= 1;
-        if (!ok) break;
-        tmem_fence_after();
-        scores(tile, done & 1);
-      }
-      if (!ok) return false;
-      umma_commit(&bars[kKEmpty + (done & 1)]);
-      for (int j = 0; ok && j < it.steps; ++j, ++done) {
-        const int stage = done & 1;
-        const uint32_t parity = (done >> 1) & 1;
-        ok = wait(kVFull + stage, parity);
-        for (int tile = 0; ok && tile < tiles; ++tile) {
-          ok = wait(kPFull + tile, p_phase[tile]);
-          p_phase[tile] ^= 1;
-          if (!ok) break;
-          tmem_fence_after();
-#pragma unroll
-          for (int x = 0; x < kPromptKeys / 16; ++x)
-            umma_ts(tmem + 256 + tile * 128, tmem + tile * 128 + x * 8,
-                    umma_desc(base + Sh::kV + stage * Sh::kTile + x * 2048, 16384, 1024), kIdescO, j > 0 || x > 0);
-          if (tile == tiles - 1) umma_commit(&bars[kVEmpty + stage]);
-          if (j + 1 < it.steps) {
-            if (tile == 0) ok = wait(kKFull + ((done + 1) & 1), ((done + 1) >> 1) & 1);
-            if (!ok) break;
-            scores(tile, (done + 1) & 1);
-            if (tile == tiles - 1) umma_commit(&bars[kKEmpty + ((done + 1) & 1)]);
-          } else {
-            umma_commit(&bars[kOFull + tile]);
-          }
-        }
-      }
-      return ok;
-    };
-    for (int64_t item = blockIdx.x; go && next_item(item); item += gridDim.x) {
-      if (it.steps == 0) continue;
-      if (lane == 0) go = run_item();
-      go = __shfl_sync(0xffffffffu, go, 0);
-    }
-    if (!go && lane == 0) {
-      // Products may be in flight over shared and tensor memory: let them end (bounded) before anything is freed.
-      umma_commit(&bars[kOFull]);
-      (void)mbar_wait_bounded(&bars[kOFull], 0, kWaitLimitNs / 4);
-    }
   }
   __syncwarp();
   tmem_fence_before();
   __syncthreads();
-  if (warp == 16) {
+  if (warp == 0) {
     tmem_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
   }

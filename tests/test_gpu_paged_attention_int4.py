@@ -1,14 +1,13 @@
 """Attention over the 4-bit cache against softmax(q k^T) v in 64 bits on the values the codes stand for.
 
 Tolerance, per element, from the kernel's arithmetic (p normalised, n keys):
-- a weight p s is rounded to fp16, 2^-11 of it, and multiplies the code c of 0..15 (bf16 results) or c - 7.5 (fp16 ones);
-  the minima's part, sum p (m + z s) with z = 0 or 7.5, has weights in fp32;
+- a weight p s is rounded to fp16, 2^-11 of it and, with the largest near 1, not below 2^-25 of the largest; it multiplies the code
+  c of 0..15 (bf16 results), c - 7.5 (fp16 ones) or c - 8 (requests with more than 64 rows a kv head); the minima's part,
+  sum p (m + z s) with z = 0, 7.5 or 8, has weights in fp32;
 - sums over n keys in fp32, by steps of 16 in the matrix unit: u = 2^-22 (n / 16 + 32) of the terms' sizes;
 - a logit is off by delta = sm_scale 2^-23 (D / 8 + 6) max_t (143 s_t + |m_t|) sum |q|: D / 16 steps of the matrix unit, two
   roundings each, and six more operations, on terms of at most 15 s |q|. It enters as 2 delta (sum p |v| + |o|);
 - the result is rounded: eps_T / 2 |o|.
-Requests with more than 64 rows a kv head take the tensor-core kernel, where u = eps_T / 2 is the rounding of the keys, of the values and of
-the weights: delta = sm_scale max_t sum |q k_t| (u + 2^-23 (D / 8 + 6)), and the weights' part is (2 u + 2^-22 (n / 16 + 32)) sum p |v|.
 """
 from __future__ import annotations
 
@@ -60,12 +59,13 @@ def _bound(q, cache, layout, table, lens, cum, scale, causal, dtype):
     out, lse = ref.attention(q, cache, layout, table, lens, cum, scale, causal)
     tol = torch.zeros_like(out)
     ltol = torch.zeros_like(lse)
-    z = 0.0 if dtype == BF else 7.5
     for b, n in enumerate(lens):
         tok = torch.arange(n)
         pages, entries = table[b].long()[tok // ps], tok % ps
         k, v = ref.read_rows(cache, layout, pages, entries)
         pr = cache[2].double()[pages, :, entries]                       # [n, h, 4]
+        # what the codes are centred on: the tensor-core kernel's rows, the other's for fp16 and for bf16
+        z = 8.0 if (cum[b + 1] - cum[b]) * (hq // h) > 64 else 0.0 if dtype == BF else 7.5
         code = (v - pr[..., 3, None]) / pr[..., 2, None]
         for i in range(cum[b], cum[b + 1]):
             seen = max(0, min(n, n - (cum[b + 1] - cum[b]) + (i - cum[b]) + 1)) if causal else n
@@ -75,20 +75,13 @@ def _bound(q, cache, layout, table, lens, cum, scale, causal, dtype):
             p = torch.softmax(torch.einsum("hgd,thd->hgt", qi, k[:seen]) * scale, -1)
             steps = 2.0 ** -22 * (seen / 16 + 32)
             weights = torch.einsum("hgt,thd->hgd", p, (code[:seen] - z).abs() * pr[:seen, :, 2, None])
+            weights = weights + 2.0 ** -14 * 15 * seen * (p * pr[:seen, :, 2].T[:, None]).amax(-1, keepdim=True)
             sums = torch.einsum("hgt,thd->hgd", p, code[:seen] * pr[:seen, :, 2, None])
             minima = torch.einsum("hgt,th->hg", p, (pr[:seen, :, 3].abs() + z * pr[:seen, :, 2]))[..., None]
             size = torch.einsum("hgt,thd->hgd", p, v[:seen].abs())
             reach = (143 * pr[:seen, :, 0] + pr[:seen, :, 1].abs()).amax(0)  # [h]
             delta = (2.0 ** -23 * (d / 8 + 6) * abs(scale) * reach[:, None] * qi.abs().sum(-1))[..., None]
             o = out[i].view(h, hq // h, d).abs()
-            if (cum[b + 1] - cum[b]) * (hq // h) > 64:
-                u = torch.finfo(dtype).eps / 2
-                terms = torch.einsum("hgd,thd->hgt", qi.abs(), k[:seen].abs()).amax(-1)
-                delta = (abs(scale) * (u + 2.0 ** -23 * (d / 8 + 6)) * terms)[..., None]
-                bound = (2 * u + steps) * size + 2 * delta * (size + o) + u * o
-                tol[i] = bound.reshape(hq, d) + torch.finfo(dtype).tiny
-                ltol[i] = (delta[..., 0] * 1.4427 + 2.0 ** -20 * (1 + lse[i].view(h, -1).abs())).reshape(hq) + steps
-                continue
             bound = 2.0 ** -11 * weights + steps * (sums + minima) + 2 * delta * (size + o) + torch.finfo(dtype).eps / 2 * o
             tol[i] = bound.reshape(hq, d) + torch.finfo(dtype).tiny
             # log2: the logits' error, the sum's and the logarithm's
