@@ -10,7 +10,7 @@
 // values' codes are centred (c - 8) so that long sums do not grow one-sidedly and cancel against the minima's part.
 //
 // Work split. The rows of a request that share a kv head (tokens x group, token-major) are cut into tiles of
-// 8, 16 or 32, the tile's keys into units; all units of a launch, requests outermost, form one line that the
+// 8 or 16, the tile's keys into units; all units of a launch, requests outermost, form one line that the
 // CTAs cut into equal shares, whatever the lengths are (they are only known on the device). A share that
 // covers a tile's keys writes the output; the others leave (sum, maximum, unnormalised o) in the
 // workspace, and a second kernel joins them in a fixed order, so results do not change from run to run.
@@ -68,8 +68,8 @@ struct AttnInt4Args {
 };
 
 // What the joining kernel needs of a tile that was split: written by the CTA whose share starts the tile.
-// {number of parts (0: nothing to join), request, the tile's first row within it, first kv head}
-constexpr int kAttnDescInts = 4;
+// {number of parts (0: nothing to join), the request's first query and queries, the tile's first row within it, first kv head}
+constexpr int kAttnDescInts = 5;
 
 // NT: the tile's rows in eights.
 __host__ __device__ constexpr int attn_part_floats(int D, int NT) { return 8 * NT * (D + 2); }
@@ -77,10 +77,10 @@ __host__ __device__ constexpr int attn_part_floats(int D, int NT) { return 8 * N
 template <int D, int NT>
 struct AttnInt4Shape {
   static constexpr int kRows = 8 * NT;
-  static constexpr int kPass = NT == 4 ? 1 : 2;  // 16-token steps a warp computes at once
-  // By registers (128, 168 and 255 a thread). At 16 rows four CTAs of 128 registers took 211 us where three take 196
+  static constexpr int kPass = 2;  // 16-token steps a warp computes at once: with one, 204 us where two take 196
+  // By registers (128 and 168 a thread). At 16 rows four CTAs of 128 registers took 211 us where three take 196
   // (spills, or half the independent products a warp), two of 255 took 221.
-  static constexpr int kCtasPerSm = NT == 1 ? 4 : NT == 2 ? 3 : 2;
+  static constexpr int kCtasPerSm = NT == 1 ? 4 : 3;
   static constexpr int kRowBytes = D / 2;
   static constexpr int kKeys = 0;
   static constexpr int kValues = kAttnRun * kRowBytes;
@@ -256,6 +256,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnInt4Shape<D, NT>::kCtasPerSm
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int64_t s_scan[kAttnWarps + 2];
   __shared__ int32_t s_b;
+  __shared__ AttnRequest s_rq;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
   uint8_t* ring = smem + Sh::kQFrag;
@@ -273,8 +274,12 @@ __global__ void __launch_bounds__(kAttnThreads, AttnInt4Shape<D, NT>::kCtasPerSm
   const int per = (a.B + kAttnThreads - 1) / kAttnThreads;
   const int rb0 = min(a.B, tid * per), rb1 = min(a.B, rb0 + per);
   int64_t mine = 0;
-  for (int b = rb0; b < rb1; ++b)
-    mine += attn_request<kRows>(a, b, blockIdx.x == 0 ? a.status : nullptr).work(head_groups);
+  AttnRequest first_rq = {};
+  for (int b = rb0; b < rb1; ++b) {
+    const AttnRequest x = attn_request<kRows>(a, b, blockIdx.x == 0 ? a.status : nullptr);
+    if (b == rb0) first_rq = x;
+    mine += x.work(head_groups);
+  }
   int64_t incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -300,17 +305,20 @@ __global__ void __launch_bounds__(kAttnThreads, AttnInt4Shape<D, NT>::kCtasPerSm
   if (at >= before && at < before + mine) {
     int64_t rem = at - before;
     int b = rb0;
+    AttnRequest mine_rq = first_rq;
     for (; b < rb1; ++b) {
-      const int64_t w = attn_request<kRows>(a, b, nullptr).work(head_groups);
+      if (b > rb0) mine_rq = attn_request<kRows>(a, b, nullptr);
+      const int64_t w = mine_rq.work(head_groups);
       if (rem < w) break;
       rem -= w;
     }
     s_b = b;
+    s_rq = mine_rq;
     s_scan[kAttnWarps] = rem;
   }
   __syncthreads();
   int b = s_b;
-  AttnRequest rq = attn_request<kRows>(a, b, nullptr);
+  AttnRequest rq = s_rq;
   int unit, head_group, tile;
   {
     int64_t rem = s_scan[kAttnWarps];
@@ -319,7 +327,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnInt4Shape<D, NT>::kCtasPerSm
     head_group = (int)(rem % head_groups);
     tile = (int)(rem / head_groups);
   }
-  int desc_parts = 0, desc_request = 0, desc_row = 0, desc_head = 0;
+  int desc_parts = 0, desc_q0 = 0, desc_qlen = 0, desc_row = 0, desc_head = 0;
 
   while (at < end) {
     // Of this share, the start's cost is passed over. A share may hold nothing but (a part of) that.
@@ -341,43 +349,6 @@ __global__ void __launch_bounds__(kAttnThreads, AttnInt4Shape<D, NT>::kCtasPerSm
     const int lim_first = limit(0);
     const uint32_t head16 = (uint32_t)(head * a.kv.stride_head >> 4);
 
-    // Queries into shared memory as the first product takes them, a warp for eight rows of a head: lane (g, t) has
-    // elements (D / 4) t and on of row g. Beside them the rows' sums and scales, two rows (2t, 2t + 1) together.
-    for (int c = warp; c < cta_heads * NT; c += kAttnWarps) {
-      const int nt = c % NT, hd = c / NT, rr = nt * 8 + g;
-      float f[D / 32][8], sum = 0.0f, most = 0.0f;
-      const int tok = (row0 + min(rr, rows_here - 1)) / a.group, sub = row0 + min(rr, rows_here - 1) - tok * a.group;
-      const uint16_t* src = static_cast<const uint16_t*>(a.q) + (int64_t)(rq.q0 + tok) * a.qsn +
-                            ((int64_t)(head_group * cta_heads + hd) * a.group + sub) * a.qsh + (D / 4) * t;
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
-        unpack8<T>(a.q_vec ? kv_load8<true>(src + 8 * i) : kv_load8<false>(src + 8 * i), f[i]);
-#pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          f[i][x] = rr < rows_here ? f[i][x] : 0.0f;
-          sum += f[i][x];
-          // as bits, so that a NaN is the most
-          most = __uint_as_float(max(__float_as_uint(most), __float_as_uint(fabsf(f[i][x]))));
-        }
-      }
-#pragma unroll
-      for (int z = 1; z < 4; z <<= 1) {
-        sum += __shfl_xor_sync(0xffffffffu, sum, z);
-        most = __uint_as_float(max(__float_as_uint(most), __shfl_xor_sync(0xffffffffu, __float_as_uint(most), z)));
-      }
-      const uint32_t exponent = min(max(__float_as_uint(most) >> 23, 12u), 254u);
-      const float scale = kRowScale ? __uint_as_float((265u - exponent) << 23) : 1.0f;
-      const float unscale = kRowScale ? __uint_as_float((exponent - 11u) << 23) : 1.0f;
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i)
-        *reinterpret_cast<uint4*>(smem + hd * Sh::kQHead + ((i * NT + nt) * 32 + lane) * 16) =
-            query_operand(f[i], scale);
-      if (t == 0) {
-        float* dst = qrow + (hd * kRows + nt * 8 + (g & ~1)) * 2 + (g & 1);
-        dst[0] = sum * scale;
-        dst[2] = unscale;
-      }
-    }
     const uint32_t qfrag_u = smem_u32(smem) + which * Sh::kQHead + lane * 16;
 
     // The warp's runs: t0 + 32 (sub_warp + head_warps * i).
@@ -432,6 +403,43 @@ __global__ void __launch_bounds__(kAttnThreads, AttnInt4Shape<D, NT>::kCtasPerSm
       const int next = load_page(i + 1);
       issue(i, page);
       page = next;
+    }
+    // Queries into shared memory as the first product takes them, a warp for eight rows of a head: lane (g, t) has
+    // elements (D / 4) t and on of row g. Beside them the rows' sums and scales, two rows (2t, 2t + 1) together.
+    for (int c = warp; c < cta_heads * NT; c += kAttnWarps) {
+      const int nt = c % NT, hd = c / NT, rr = nt * 8 + g;
+      float f[D / 32][8], sum = 0.0f, most = 0.0f;
+      const int tok = (row0 + min(rr, rows_here - 1)) / a.group, sub = row0 + min(rr, rows_here - 1) - tok * a.group;
+      const uint16_t* src = static_cast<const uint16_t*>(a.q) + (int64_t)(rq.q0 + tok) * a.qsn +
+                            ((int64_t)(head_group * cta_heads + hd) * a.group + sub) * a.qsh + (D / 4) * t;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        unpack8<T>(a.q_vec ? kv_load8<true>(src + 8 * i) : kv_load8<false>(src + 8 * i), f[i]);
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          f[i][x] = rr < rows_here ? f[i][x] : 0.0f;
+          sum += f[i][x];
+          // as bits, so that a NaN is the most
+          most = __uint_as_float(max(__float_as_uint(most), __float_as_uint(fabsf(f[i][x]))));
+        }
+      }
+#pragma unroll
+      for (int z = 1; z < 4; z <<= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, z);
+        most = __uint_as_float(max(__float_as_uint(most), __shfl_xor_sync(0xffffffffu, __float_as_uint(most), z)));
+      }
+      const uint32_t exponent = min(max(__float_as_uint(most) >> 23, 12u), 254u);
+      const float scale = kRowScale ? __uint_as_float((265u - exponent) << 23) : 1.0f;
+      const float unscale = kRowScale ? __uint_as_float((exponent - 11u) << 23) : 1.0f;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+        *reinterpret_cast<uint4*>(smem + hd * Sh::kQHead + ((i * NT + nt) * 32 + lane) * 16) =
+            query_operand(f[i], scale);
+      if (t == 0) {
+        float* dst = qrow + (hd * kRows + nt * 8 + (g & ~1)) * 2 + (g & 1);
+        dst[0] = sum * scale;
+        dst[2] = unscale;
+      }
     }
     __syncthreads();  // the queries are in shared memory
 
@@ -804,7 +812,8 @@ __global__ void __launch_bounds__(kAttnThreads, AttnInt4Shape<D, NT>::kCtasPerSm
       // The tile goes on in the following CTAs, up to the one that holds its last unit.
       const int64_t last = (at + rq.units - 1) / share;
       desc_parts = (int)(last - blockIdx.x) + 1;
-      desc_request = b;
+      desc_q0 = rq.q0;
+      desc_qlen = rq.qlen;
       desc_row = row0;
       desc_head = head_group * cta_heads;
     }
@@ -825,9 +834,10 @@ __global__ void __launch_bounds__(kAttnThreads, AttnInt4Shape<D, NT>::kCtasPerSm
   }
   if (tid == 0 && a.desc != nullptr) {
     desc[0] = desc_parts;
-    desc[1] = desc_request;
-    desc[2] = desc_row;
-    desc[3] = desc_head;
+    desc[1] = desc_q0;
+    desc[2] = desc_qlen;
+    desc[3] = desc_row;
+    desc[4] = desc_head;
   }
   pdl_launch_dependents();
 }
@@ -844,9 +854,8 @@ __global__ void __launch_bounds__(kAttnThreads) attn_int4_join_kernel(const Attn
   const int32_t* desc = a.desc + (int64_t)blockIdx.x * kAttnDescInts;
   const int parts = desc[0];
   if (parts > 0) {
-    const AttnRequest rq = attn_request<kRows>(a, desc[1], nullptr);
-    const int row = desc[2] + r, head = desc[3] + which;
-    if (row < rq.qlen * a.group) {
+    const int q0 = desc[1], row = desc[3] + r, head = desc[4] + which;
+    if (row < desc[2] * a.group) {
       constexpr int kPer = D / 32;
       const int64_t slot = (int64_t)a.cta_heads * attn_part_floats(D, NT);
       // part 0 is slot 1 of CTA c, part i slot 0 of CTA c + i
@@ -871,12 +880,12 @@ __global__ void __launch_bounds__(kAttnThreads) attn_int4_join_kernel(const Attn
       }
       const int tok = row / a.group, sub = row - tok * a.group;
       const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
-      uint16_t* dst = static_cast<uint16_t*>(a.out) + (int64_t)(rq.q0 + tok) * a.osn +
+      uint16_t* dst = static_cast<uint16_t*>(a.out) + (int64_t)(q0 + tok) * a.osn +
                       ((int64_t)head * a.group + sub) * a.osh;
 #pragma unroll
       for (int j = 0; j < kPer; ++j) dst[j * 32 + lane] = Elem<T>::from_f(acc[j] * inv);
       if (lane == 0 && a.lse != nullptr)
-        a.lse[(int64_t)(rq.q0 + tok) * a.kv.heads * a.group + (int64_t)head * a.group + sub] =
+        a.lse[(int64_t)(q0 + tok) * a.kv.heads * a.group + (int64_t)head * a.group + sub] =
             sum != 0.0f ? top + __log2f(sum) : -INFINITY;
     }
   }

@@ -37,7 +37,10 @@ constexpr int kPromptThreads = 512;
 constexpr int kPromptSoftmaxRegs = 168, kPromptUnpackRegs = 88;
 constexpr int kPromptRows = 256;  // rows of a CTA's item
 constexpr int kPromptKeys = 128;  // keys of a step
-constexpr int kAttnSplitRows = 64;  // requests with more rows a kv head go to this kernel
+// Requests with more rows a kv head go to this kernel, in calls with enough rows to give the SMs work without cutting contexts.
+// 16 requests over 4 K tokens (96/8 heads), this kernel against tiles of 16 rows: 72 rows 144 and 115 us, 96 rows 146 and 135,
+// 132 rows (114 a SM in all) 188 and 192, 192 rows (166 a SM) 192 and 248.
+constexpr int kAttnSplitRows = 96, kPromptRowsPerSm = 160;
 
 template <int D>
 struct PromptShape {

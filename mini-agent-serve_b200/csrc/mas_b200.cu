@@ -120,10 +120,8 @@ cudaError_t opt_in_attn_int4() {
   if ((e = opt_in_smem(attn_int4_prompt_kernel<T, 128>, PromptShape<128>::kSmem)) != cudaSuccess) return e;
   if ((e = opt_in_smem(attn_int4_kernel<T, 64, 1>, AttnInt4Shape<64, 1>::kSmem)) != cudaSuccess) return e;
   if ((e = opt_in_smem(attn_int4_kernel<T, 64, 2>, AttnInt4Shape<64, 2>::kSmem)) != cudaSuccess) return e;
-  if ((e = opt_in_smem(attn_int4_kernel<T, 64, 4>, AttnInt4Shape<64, 4>::kSmem)) != cudaSuccess) return e;
   if ((e = opt_in_smem(attn_int4_kernel<T, 128, 1>, AttnInt4Shape<128, 1>::kSmem)) != cudaSuccess) return e;
-  if ((e = opt_in_smem(attn_int4_kernel<T, 128, 2>, AttnInt4Shape<128, 2>::kSmem)) != cudaSuccess) return e;
-  return opt_in_smem(attn_int4_kernel<T, 128, 4>, AttnInt4Shape<128, 4>::kSmem);
+  return opt_in_smem(attn_int4_kernel<T, 128, 2>, AttnInt4Shape<128, 2>::kSmem);
 }
 
 cudaError_t prepare_current(DeviceState& st, int device) {
@@ -717,17 +715,17 @@ int run_kv_int4(KVInt4RowArgs a, const MasInt4KVCache* cache, int64_t num_kv_hea
 // The workspace of an attention launch: every CTA's two parts, then its descriptor; sized for the tile height
 // that needs most.
 int64_t attn_ctas(const DeviceState& st, int NT) {
-  return (int64_t)st.sm_count * (NT == 1 ? AttnInt4Shape<128, 1>::kCtasPerSm
-                                         : NT == 2 ? AttnInt4Shape<128, 2>::kCtasPerSm : AttnInt4Shape<128, 4>::kCtasPerSm);
+  return (int64_t)st.sm_count * (NT == 1 ? AttnInt4Shape<128, 1>::kCtasPerSm : AttnInt4Shape<128, 2>::kCtasPerSm);
 }
 int64_t attn_part_bytes(const DeviceState& st, int64_t head_size) {
   int64_t most = 0;
-  for (int nt = 1; nt <= 4; nt *= 2)
+  for (int nt = 1; nt <= 2; ++nt)
     most = std::max(most, attn_ctas(st, nt) * 2 * kAttnMaxHeads * attn_part_floats((int)head_size, nt));
   return most * (int64_t)sizeof(float);
 }
 int64_t attn_workspace_bytes(const DeviceState& st, int64_t head_size) {
-  return attn_part_bytes(st, head_size) + std::max({attn_ctas(st, 1), attn_ctas(st, 2), attn_ctas(st, 4)}) * kAttnDescInts * (int64_t)sizeof(int32_t);
+  return attn_part_bytes(st, head_size) +
+         std::max(attn_ctas(st, 1), attn_ctas(st, 2)) * kAttnDescInts * (int64_t)sizeof(int32_t);
 }
 
 template <typename T, int D, int NT>
@@ -750,23 +748,27 @@ int launch_attn_int4(AttnInt4Args a, DeviceState* st, void* stream, int enable_p
 
 template <typename T, int D>
 int run_attn_int4(AttnInt4Args a, DeviceState* st, void* stream, int enable_pdl) {
-  // Rows that share a request's kv head, on average. The lengths are the device's: where some request may have more
+  // Rows that share a request's kv head, on average: tiles of 8 rows where they do, of 16 otherwise (drafts of 8 to 32 rows
+  // over 4 K tokens: 164 us with 8, 147 with 16, 193 with tiles of 32, which are not built; 12 rows: 253, 186 and 348; one row:
+  // 27, 33 and 49). The lengths are the device's: where some request may have more
   // than split_rows rows, the prompt kernel is launched for those and this one leaves them out; both may find nothing.
   int64_t rows = ceil_div(a.T, a.B) * a.group;
-  static const int env_split = env_int("MAS_ATTN_SPLIT_ROWS", kAttnSplitRows);
   a.split_rows = INT32_MAX;
-  if (a.cum_q != nullptr && a.T * a.group > env_split) {
-    a.split_rows = env_split;
+  // Where some request may have more than kAttnSplitRows rows, the prompt kernel is launched for those and this one leaves
+  // them out; both may find nothing. The prompt kernel does not cut contexts, so it needs items: 160 rows an SM.
+  static const int env_min = env_int("MAS_ATTN_PROMPT_MIN_ROWS", -1);
+  const int64_t min_rows = env_min >= 0 ? env_min : (int64_t)kPromptRowsPerSm * st->sm_count;
+  if (a.cum_q != nullptr && a.T * a.group > kAttnSplitRows && a.T * a.group * a.kv.heads >= min_rows) {
+    a.split_rows = kAttnSplitRows;
     const int64_t items = (ceil_div(a.T * a.group, kPromptRows) + a.B) * a.kv.heads;
     const unsigned grid = (unsigned)std::min<int64_t>(items, st->sm_count);
     const int rc = launch(attn_int4_prompt_kernel<T, D>, dim3(grid), dim3(kPromptThreads), PromptShape<D>::kSmem, stream,
                           enable_pdl, a, st->fault);
     if (rc != MAS_OK) return rc;
-    if (rows > env_split) rows = a.group;  // prompts in the mean: what is left are decode rows
+    if (rows > kAttnSplitRows) rows = a.group;  // prompts in the mean: what is left are decode rows
   }
   if (rows <= 8) return launch_attn_int4<T, D, 1>(a, st, stream, enable_pdl);
-  if (rows <= 16) return launch_attn_int4<T, D, 2>(a, st, stream, enable_pdl);
-  return launch_attn_int4<T, D, 4>(a, st, stream, enable_pdl);
+  return launch_attn_int4<T, D, 2>(a, st, stream, enable_pdl);
 }
 
 }  // namespace

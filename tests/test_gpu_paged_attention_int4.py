@@ -2,7 +2,7 @@
 
 Tolerance, per element, from the kernel's arithmetic (p normalised, n keys):
 - a weight p s is rounded to fp16, 2^-11 of it and, with the largest near 1, not below 2^-25 of the largest; it multiplies the code
-  c of 0..15 (bf16 results), c - 7.5 (fp16 ones) or c - 8 (requests with more than 64 rows a kv head); the minima's part,
+  c of 0..15 (bf16 results), c - 7.5 (fp16 ones) or c - 8 (the prompt kernel); the minima's part,
   sum p (m + z s) with z = 0, 7.5 or 8, has weights in fp32;
 - sums over n keys in fp32, by steps of 16 in the matrix unit: u = 2^-22 (n / 16 + 32) of the terms' sizes;
 - a logit is off by delta = sm_scale 2^-23 (D / 8 + 6) max_t (143 s_t + |m_t|) sum |q|: D / 16 steps of the matrix unit, two
@@ -12,7 +12,11 @@ Tolerance, per element, from the kernel's arithmetic (p normalised, n keys):
 from __future__ import annotations
 
 import math
+import os
 import random
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -52,6 +56,13 @@ def _make(seed, lens, hkv, d, page_size, layout, poison=True, v_scale=1.0):
     return (codes[0], codes[1], pairs), table
 
 
+def _takes_prompt_kernel(tokens: int, hq: int, rows: int) -> bool:
+    """The library's choice for a request with that many rows a kv head."""
+    least = os.environ.get("MAS_ATTN_PROMPT_MIN_ROWS")
+    least = int(least) if least else 160 * torch.cuda.get_device_properties(0).multi_processor_count
+    return rows > 96 and tokens * hq >= least
+
+
 def _bound(q, cache, layout, table, lens, cum, scale, causal, dtype):
     """The 64-bit result, its lse, the tolerance, and the rows some request covers."""
     T, hq, d = q.shape
@@ -65,7 +76,9 @@ def _bound(q, cache, layout, table, lens, cum, scale, causal, dtype):
         k, v = ref.read_rows(cache, layout, pages, entries)
         pr = cache[2].double()[pages, :, entries]                       # [n, h, 4]
         # what the codes are centred on: the tensor-core kernel's rows, the other's for fp16 and for bf16
-        z = 8.0 if (cum[b + 1] - cum[b]) * (hq // h) > 64 else 0.0 if dtype == BF else 7.5
+        z = 0.0 if dtype == BF else 7.5
+        if _takes_prompt_kernel(T, hq, (cum[b + 1] - cum[b]) * (hq // h)):
+            z = 8.0
         code = (v - pr[..., 3, None]) / pr[..., 2, None]
         for i in range(cum[b], cum[b + 1]):
             seen = max(0, min(n, n - (cum[b + 1] - cum[b]) + (i - cum[b]) + 1)) if causal else n
@@ -177,6 +190,22 @@ def test_prompt_rows_of_odd_pages_and_scales(cuda, causal):
     _run(64, [333], [150], 6, 2, 64, BF, page_size=1, causal=causal, q_gain=30.0)
     _run(65, [500], [40], 6, 2, 128, FP, causal=causal, v_scale=1e-4)
     _run(66, [500], [40], 6, 2, 128, BF, causal=causal, v_scale=1e30)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_prompt_rows_beside_decode_rows(cuda, dtype):
+    """A mixed step at the 123B-class head counts, large enough for the prompt kernel by itself."""
+    _run(69, [450, 77, 300, 1, 130], [190, 1, 80, 1, 2], 96, 8, 128, dtype)
+
+
+def test_small_prompts_through_the_prompt_kernel(cuda):
+    """The prompt tests again in a process where the prompt kernel takes calls of any size."""
+    env = dict(os.environ, MAS_ATTN_PROMPT_MIN_ROWS="0")
+    here = Path(__file__).resolve()
+    r = subprocess.run([sys.executable, "-m", "pytest", str(here), "-x", "-q", "-m", "gpu", "-k",
+                        "prompt_rows or ragged or random_shapes or hidden_nan or decode_loop"], env=env, cwd=here.parents[1],
+                       capture_output=True, text=True, timeout=600)
+    assert r.returncode == 0, r.stdout[-3000:] + r.stderr[-2000:]
 
 
 def test_prompt_rows_over_many_items_and_requests(cuda):
