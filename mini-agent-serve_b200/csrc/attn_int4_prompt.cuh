@@ -6,8 +6,8 @@
 // run on bare codes (c - 8 in fp16, exact) and the pairs enter in fp32, between them:
 //   y = S' ks + (sum q) kb,  p = 2^(y - M),  l += p,  r += p (mv + 8 sv),  w = fp16(p sv),  O += w (cv - 8),  o = (O + r) / l
 // (ks, kb the key's scale and minimum + 8 scales, times the softmax scale and log2 e). Keys and values rounded to bf16 on the
-// way in, which needs two of these eight instructions less a (row, key), took 924 us at the case below, but were 0.0051 of the
-// result off where this is 0.0018. M is one reference for all: the row's largest log2 of a weight p sv, moved when one passes it by 8.
+// way in, which needs two of these eight instructions less a (row, key), took 924 us for 2 requests of 700 to 2048 new tokens over
+// up to 8 K (96/8 heads of 128) where this takes 1390, but were 0.0051 of the result off where this is 0.0017. M is one reference for all: the row's largest log2 of a weight p sv, moved when one passes it by 8.
 //
 // A CTA takes 256 rows of one kv head (two tiles of 128, the height of an MMA) and walks the keys in steps of 128:
 //   warps 8-15   unpack a step's codes into shared memory, a thread a key: K [key][D] (8-11) and V [key][D] (12-15), 128-byte
@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
     s_stop = 0;
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars[kKFull + i], 128);
-      mbar_init(&bars[kKEmpty + i], 2);  // each tile's products, or one tile's twice
+      mbar_init(&bars[kKEmpty + i], 2);  // each tile's products
       mbar_init(&bars[kVFull + i], 128);
       mbar_init(&bars[kVEmpty + i], 2);
       mbar_init(&bars[kSFull + i], 1);
@@ -284,10 +284,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
     // Products, by one thread a tile. Step d (of all items) uses stage d & 1.
     constexpr uint32_t kIdescS = umma_idesc(128, kPromptKeys, false), kIdescO = umma_idesc(128, D, true);
     const bool issuer = lane == 0 && (warp & 3) == 0;
-    auto release = [&](int bar) {  // of a stage: with one tile at work its products stand for the other's, too
-      umma_commit(&bars[bar]);
-      if (it.rows <= 128) umma_commit(&bars[bar]);
-    };
     auto issue_scores = [&](uint32_t d) {
       const int stage = d & 1;
       if (!wait(kKFull + stage, (d >> 1) & 1)) return;
@@ -299,7 +295,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
         umma_ss(tmem + tile * 128, umma_desc(q + off, 16, 1024), umma_desc(k + off, 16, 1024), kIdescS, x > 0);
       }
       umma_commit(&bars[kSFull + tile]);
-      release(kKEmpty + stage);
+      umma_commit(&bars[kKEmpty + stage]);
     };
     auto issue_values = [&](uint32_t d, bool accumulate) {
       const int stage = d & 1;
@@ -309,13 +305,23 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
       for (int x = 0; x < kPromptKeys / 16; ++x)
         umma_ts(tmem + 256 + tile * 128, tmem + tile * 128 + x * 8,
                 umma_desc(base + Sh::kV + stage * Sh::kTile + x * 2048, 16384, 1024), kIdescO, accumulate || x > 0);
-      release(kVEmpty + stage);
+      umma_commit(&bars[kVEmpty + stage]);
     };
     uint32_t s_phase = 0, o_phase = 0, p_phase = 0, q_phase = 0;
     uint32_t done = 0;  // steps so far, over all items, this tile's rows at work or not
     bool go = true;
     for (int64_t item = blockIdx.x; go && next_item(item); item += gridDim.x) {
       if (tile * 128 >= it.rows) {
+        // No rows: the tile still takes and gives back each stage, or it would meet the next item's barriers phases early.
+        for (int j = 0; issuer && j < it.steps; ++j) {
+          const int stage = (done + j) & 1;
+          const uint32_t parity = ((done + j) >> 1) & 1;
+          if (!wait(kKFull + stage, parity)) break;
+          mbar_arrive(&bars[kKEmpty + stage]);
+          if (!wait(kVFull + stage, parity)) break;
+          mbar_arrive(&bars[kVEmpty + stage]);
+        }
+        __syncwarp();
         done += it.steps;
         continue;
       }

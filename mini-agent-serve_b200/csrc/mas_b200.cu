@@ -750,12 +750,11 @@ template <typename T, int D>
 int run_attn_int4(AttnInt4Args a, DeviceState* st, void* stream, int enable_pdl) {
   // Rows that share a request's kv head, on average: tiles of 8 rows where they do, of 16 otherwise (drafts of 8 to 32 rows
   // over 4 K tokens: 164 us with 8, 147 with 16, 193 with tiles of 32, which are not built; 12 rows: 253, 186 and 348; one row:
-  // 27, 33 and 49). The lengths are the device's: where some request may have more
-  // than split_rows rows, the prompt kernel is launched for those and this one leaves them out; both may find nothing.
+  // 27, 33 and 49).
   int64_t rows = ceil_div(a.T, a.B) * a.group;
   a.split_rows = INT32_MAX;
-  // Where some request may have more than kAttnSplitRows rows, the prompt kernel is launched for those and this one leaves
-  // them out; both may find nothing. The prompt kernel does not cut contexts, so it needs items: 160 rows an SM.
+  // The lengths are the device's: where some request may have more than kAttnSplitRows rows, the prompt kernel is launched
+  // for those and this one leaves them out; both may find nothing. The prompt kernel does not cut contexts, so it needs items: 160 rows an SM.
   static const int env_min = env_int("MAS_ATTN_PROMPT_MIN_ROWS", -1);
   const int64_t min_rows = env_min >= 0 ? env_min : (int64_t)kPromptRowsPerSm * st->sm_count;
   if (a.cum_q != nullptr && a.T * a.group > kAttnSplitRows && a.T * a.group * a.kv.heads >= min_rows) {

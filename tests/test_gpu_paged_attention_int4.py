@@ -215,6 +215,15 @@ def test_prompt_rows_over_many_items_and_requests(cuda):
     _run(67, lens, qlens, 16, 4, 64, BF)
 
 
+@pytest.mark.parametrize("seed", range(3))
+def test_prompt_items_of_one_tile_before_items_of_two(cuda, seed):
+    """Each CTA meets items of up to 128 rows, at many steps, between larger ones: the idle tile keeps its place."""
+    rng = random.Random(70 + seed)
+    qlens = [rng.choice([60, 64, 65, 100, 160, 200]) for _ in range(60)]  # 120 to 400 rows a kv head
+    lens = [n + rng.choice([0, 130, 700, 1300]) for n in qlens]
+    _run(71 + seed, lens, qlens, 16, 8, 64, BF)
+
+
 def test_hidden_nan_keys_do_not_reach_earlier_prompt_rows(cuda):
     lens, qlens = [150], [100]
     cache, table = _make(68, lens, 2, 128, 16, "NHD")
