@@ -426,8 +426,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
               cand = fmaxf(cand, fmaxf(fmaf(__uint_as_float(s[i]), unscale, lv.x), fmaf(__uint_as_float(s[i + 1]), unscale, lv.y)));
             }
           }
-          // Values of scale 0 (or next to it) weigh nothing, but p is to stay finite. (Scales past 2^100 would cost l small p's.)
-          cand = fmaxf(cand, top - 100.0f);
+          // Values of next to no scale (a constant row's is 2^-126) weigh nothing, but their minima do: p stays below 2^68, so
+          // that r holds minima up to 2^40 or so, while scales down to 2^-60 keep their weights' bits.
+          cand = fmaxf(cand, top - 60.0f);
           const bool up = cand > m + 8.0f;
           if (__any_sync(0xffffffffu, up)) {
             const float was = m;

@@ -224,6 +224,44 @@ def test_prompt_items_of_one_tile_before_items_of_two(cuda, seed):
     _run(71 + seed, lens, qlens, 16, 8, 64, BF)
 
 
+@pytest.mark.parametrize("value", [-1.0, 1500.0, 1e9])
+@pytest.mark.parametrize("tokens,new", [(2000, 1), (2000, 8), (2000, 1500)])
+def test_constant_values(cuda, tokens, new, value):
+    """Value rows without a spread have the smallest scale; the result is their minimum, whatever the weights are. Off by the
+    result's rounding (2^-8) and the sums' (2^-22 (2000 / 16 + 32) < 2^-14)."""
+    heads = 2
+    cache = mas_b200.empty_paged_kv_cache_int4(tokens // 16 + 1, 16, heads, 128)
+    table = torch.arange(tokens // 16 + 1, dtype=torch.int32, device="cuda")[None]
+    g = torch.Generator(device="cuda").manual_seed(3)
+    k = torch.randn(tokens, heads, 128, generator=g, device="cuda").to(BF)
+    v = torch.full_like(k, value)
+    mas_b200.append_paged_kv_cache_int4(k, v, torch.zeros(tokens, dtype=torch.int32, device="cuda"),
+                                        torch.arange(tokens, dtype=torch.int32, device="cuda"), cache, table.flatten(),
+                                        torch.tensor([0, table.shape[1]], dtype=torch.int32, device="cuda"),
+                                        torch.tensor([16], dtype=torch.int32, device="cuda"))
+    q = torch.randn(new, 16, 128, generator=g, device="cuda").to(BF)
+    out = mas_b200.paged_attention_int4(q, cache, table, torch.tensor([tokens], dtype=torch.int32, device="cuda"),
+                                        torch.tensor([0, new], dtype=torch.int32, device="cuda"))
+    want = v[0, 0, 0].double()
+    assert ((out.double() - want).abs() <= (2.0 ** -8 + 2.0 ** -14) * want.abs()).all()
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_tensors_on_another_device_than_the_current(cuda):
+    """One step's operators on cuda:1 while cuda:0 is current."""
+    dev = torch.device("cuda:1")
+    lens, qlens = [70, 5], [1, 2]
+    cache, table = _make(77, lens, 2, 128, 16, "NHD")
+    q = torch.randn(3, 8, 128).to(BF)
+    i32 = dict(dtype=torch.int32)
+    args = (table, torch.tensor(lens, **i32), torch.tensor([0, 1, 3], **i32))
+    want = mas_b200.paged_attention_int4(q.cuda(0), tuple(t.cuda(0) for t in cache), *[t.cuda(0) for t in args])
+    got = mas_b200.paged_attention_int4(q.to(dev), tuple(t.to(dev) for t in cache), *[t.to(dev) for t in args])
+    assert torch.cuda.current_device() == 0
+    torch.cuda.synchronize(dev)
+    assert_bits_equal(got.cpu(), want.cpu(), "cuda:1")
+
+
 def test_hidden_nan_keys_do_not_reach_earlier_prompt_rows(cuda):
     lens, qlens = [150], [100]
     cache, table = _make(68, lens, 2, 128, 16, "NHD")
