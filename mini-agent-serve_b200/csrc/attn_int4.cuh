@@ -2,12 +2,12 @@
 //
 // With k_t = ck_t sk_t + mk_t and v_t = cv_t sv_t + mv_t (kv_int4.cuh), a query row q sees
 //   S_t = scale * (sk_t * sum_d q_d ck_td + mk_t * sum_d q_d)            (t up to the row's causal limit)
-//   o_d = (sum_t p_t sv_t (cv_td - 8) + sum_t p_t (mv_t + 8 sv_t)) / sum_t p_t,   p_t = exp(S_t - max S)
+//   o_d = (sum_t p_t sv_t (cv_td - z) + sum_t p_t (mv_t + z sv_t)) / sum_t p_t,   p_t = exp(S_t - max S)
 // so the matrix products run on the bare codes, exact in 16 bits, and the pairs enter per token in fp32:
 // no key or value is ever rounded. The weights w_t = p_t sv_t are rounded to fp16 for the second product (11 bits
 // where bf16 has 8, whatever the queries' type); their own running reference, apart from the logits', keeps the
-// largest of a row near 1 whatever the scales are. Maxima, sums and products are accumulated in fp32. The
-// values' codes are centred (c - 8) so that long sums do not grow one-sidedly and cancel against the minima's part.
+// largest of a row near 1 whatever the scales are. Maxima, sums and products are accumulated in fp32. z is 0
+// for bf16 results and 7.5 for fp16 ones, where the weights' rounding counts: it then meets codes of half the size.
 //
 // Work split. The rows of a request that share a kv head (tokens x group, token-major) are cut into tiles of
 // 8 or 16, the tile's keys into units; all units of a launch, requests outermost, form one line that the
@@ -24,6 +24,10 @@
 // the rows as its 8 columns, so tiles come in steps of 8 rows and a lane's operands come straight from the
 // staged bytes: the D axis is permuted so that a lane's codes are 16 (8) consecutive bytes of a row. The weights
 // leave the first product's layout for the second's operand by one 8x8 transpose (movmatrix) each.
+//
+// Measured (96/8 heads of 128, graph replays): 256 requests of up to 4 K tokens, a query each, 185 us against a floor of 88
+// (bytes); 48 of up to 8 K with 2 to 8 drafts each (32/8 heads, fp16) 140 (37); what bounds it is issue: 740 warp instructions a run of 32 tokens of a head, 51 % of the
+// slots with 12 warps an SM, ALU 42 %, tensor pipe 35 %, DRAM 37 %. 12 heads of 64 with one row each: 27 us (6), latency.
 #pragma once
 
 #include <type_traits>

@@ -5,9 +5,14 @@
 // brings in, so the products decide, 4 * D flops a row and key, and each key is unpacked once for 256 rows. Here, too, the products
 // run on bare codes (c - 8 in fp16, exact) and the pairs enter in fp32, between them:
 //   y = S' ks + (sum q) kb,  p = 2^(y - M),  l += p,  r += p (mv + 8 sv),  w = fp16(p sv),  O += w (cv - 8),  o = (O + r) / l
-// (ks, kb the key's scale and minimum + 8 scales, times the softmax scale and log2 e). Keys and values rounded to bf16 on the
-// way in, which needs two of these eight instructions less a (row, key), took 924 us for 2 requests of 700 to 2048 new tokens over
-// up to 8 K (96/8 heads of 128) where this takes 1390, but were 0.0051 of the result off where this is 0.0017. M is one reference for all: the row's largest log2 of a weight p sv, moved when one passes it by 8.
+// (ks, kb the key's scale and minimum + 8 scales, times the softmax scale and log2 e). M is one reference for all: the row's
+// largest log2 of a weight p sv, moved when one passes it by 8.
+//
+// Measured: 911 and 1511 new tokens of 6 K (96/8 heads of 128) take 1385 us against a floor of 393 (products). What bounds it is the
+// softmax warps, two a scheduler, which issue in 36 % of the cycles: without their arithmetic 749 us, without exponentials 1294,
+// without factor loads 1213. Sixteen softmax warps of half a row a thread took 1798 (104 registers spill), two S buffers of 64 keys a
+// tile 15 % more than this. Keys and values rounded to bf16 on the way in, two instructions less a (row, key), took 924, but were
+// 0.0051 of the result off where this is 0.0017.
 //
 // A CTA takes 256 rows of one kv head (two tiles of 128, the height of an MMA) and walks the keys in steps of 128:
 //   warps 8-15   unpack a step's codes into shared memory, a thread a key: K [key][D] (8-11) and V [key][D] (12-15), 128-byte

@@ -162,6 +162,8 @@ __device__ __forceinline__ void kv_store8(uint16_t* p, const Vec16& v) {
 // 8 elements a lane, so a row's minimum and maximum are a few shuffles away and its codes leave as one
 // 4-byte word a lane. A warp takes up to kKVInt4Unroll passes of one token, all their loads first
 // (grid: x over tokens, y over its groups of heads, so that no index is divided).
+// What bounds it is issue, not bytes: 168 warp instructions a (token, head) of 128, 63 % of the issue slots and 61 % of the
+// ALU's; 38 K tokens of 8 heads take 67 us (floor 30 us at 6.5 TB/s), 73 with an index division a row.
 template <typename T, typename PosT, int D, bool ALIGNED>
 __global__ void __launch_bounds__(kKVInt4Threads) append_kv_int4_kernel(const KVInt4RowArgs a) {
   constexpr int kLanes = D / 8;               // lanes a row
@@ -238,7 +240,8 @@ __device__ __forceinline__ float kv_top() {
   return std::is_same<T, __half>::value ? 65504.0f : 3.38953139e38f;
 }
 
-// The read-back: the same lanes, 4 bytes of codes in and 16 bytes of values out each.
+// The read-back: the same lanes, 4 bytes of codes in and 16 bytes of values out each. 38 K tokens of 8 heads of 128: 44 us
+// (floor 30), by issue again (59 %, ALU 64 %).
 template <typename T, typename PosT, int D, bool ALIGNED>
 __global__ void __launch_bounds__(kKVInt4Threads) read_kv_int4_kernel(const KVInt4RowArgs a) {
   constexpr int kLanes = D / 8;
