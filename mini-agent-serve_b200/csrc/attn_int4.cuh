@@ -75,9 +75,10 @@ struct AttnInt4Args {
 // {number of parts (0: nothing to join), the request's first query and queries, the tile's first row within it, first kv head}
 constexpr int kAttnDescInts = 5;
 
-// NT: the tile's rows in eights.
-__host__ __device__ constexpr int attn_part_floats(int D, int NT) { return 8 * NT * (D + 2); }
+// A part of a tile: its rows' unnormalised o, then {maximum, sum} of each.
+__host__ __device__ constexpr int attn_part_floats(int D, int rows) { return rows * (D + 2); }
 
+// NT: the tile's rows in eights.
 template <int D, int NT>
 struct AttnInt4Shape {
   static constexpr int kRows = 8 * NT;
@@ -755,7 +756,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnInt4Shape<D, NT>::kCtasPerSm
     __syncthreads();
     const bool starts = unit == 0, ends = unit + seg_units == rq.units;
     const int slot = starts && !ends ? 1 : 0;
-    float* part = a.part + (((int64_t)blockIdx.x * 2 + slot) * cta_heads + which) * attn_part_floats(D, NT);
+    float* part = a.part + (((int64_t)blockIdx.x * 2 + slot) * cta_heads + which) * attn_part_floats(D, kRows);
     const int first_warp = which * head_warps;
     // This warp's share of the D tiles.
     const int tiles_here = kMt / head_warps;
@@ -848,9 +849,8 @@ __global__ void __launch_bounds__(kAttnThreads, AttnInt4Shape<D, NT>::kCtasPerSm
 
 // Joins the parts of the tiles that were split: CTA (c, y) takes four (head, row) pairs of the tile that the
 // main kernel's CTA c started, a warp each, in the order of the parts.
-template <typename T, int D, int NT>
+template <typename T, int D, int kRows>
 __global__ void __launch_bounds__(kAttnThreads) attn_int4_join_kernel(const AttnInt4Args a) {
-  constexpr int kRows = 8 * NT;
   pdl_wait();
   const int lane = threadIdx.x & 31;
   const int hr = blockIdx.y * kAttnWarps + (threadIdx.x >> 5);
@@ -861,9 +861,9 @@ __global__ void __launch_bounds__(kAttnThreads) attn_int4_join_kernel(const Attn
     const int q0 = desc[1], row = desc[3] + r, head = desc[4] + which;
     if (row < desc[2] * a.group) {
       constexpr int kPer = D / 32;
-      const int64_t slot = (int64_t)a.cta_heads * attn_part_floats(D, NT);
+      const int64_t slot = (int64_t)a.cta_heads * attn_part_floats(D, kRows);
       // part 0 is slot 1 of CTA c, part i slot 0 of CTA c + i
-      const float* rest = a.part + blockIdx.x * 2 * slot + which * attn_part_floats(D, NT);
+      const float* rest = a.part + blockIdx.x * 2 * slot + which * attn_part_floats(D, kRows);
       const float* first = rest + slot;
       float top = -INFINITY;
       for (int i = lane; i < parts; i += 32)

@@ -167,11 +167,33 @@ __device__ __forceinline__ void unpack_row(uint32_t base, int row, const uint32_
   }
 }
 
-// An item of work: 256 rows of one kv head of one request.
+// What starting on an item costs (its queries, the first loads' latency), in steps, and the fewest steps of a share.
+constexpr int kPromptLead = 2, kPromptMinShare = 8;
+
+// A stretch of the line of work: steps u0 .. u1 of an item, 256 rows of one kv head of one request.
 struct PromptItem {
   AttnRequest rq;
-  int32_t b, head, row0, rows, steps;
+  int32_t b, head, block;  // the block of rows
+  int32_t row0, rows, u0, u1;
+  int32_t starts, ends;    // the item's first, last step is in it
 };
+
+// Steps of 128 keys that a block of rows sees.
+__device__ __forceinline__ int prompt_steps(const AttnInt4Args& a, const AttnRequest& rq, int block) {
+  const int rows = min((block + 1) * kPromptRows, rq.qlen * a.group);
+  const int seen = a.causal ? min(rq.n, max(0, rq.n - rq.qlen + (rows - 1) / a.group + 1)) : rq.n;
+  return (seen + kPromptKeys - 1) / kPromptKeys;
+}
+__device__ __forceinline__ int prompt_blocks(const AttnInt4Args& a, const AttnRequest& rq) {
+  const int64_t rows = (int64_t)rq.qlen * a.group;
+  return rows > a.split_rows ? (int)((rows + kPromptRows - 1) / kPromptRows) : 0;
+}
+// A kv head's work of a request: of each block its steps, at least one, and the lead.
+__device__ __forceinline__ int64_t prompt_work(const AttnInt4Args& a, const AttnRequest& rq) {
+  int64_t work = 0;
+  for (int k = prompt_blocks(a, rq) - 1; k >= 0; --k) work += max(1, prompt_steps(a, rq, k)) + kPromptLead;
+  return work;
+}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(const AttnInt4Args a, int32_t* fault) {
@@ -183,56 +205,102 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
   uint8_t* shared = raw + (base - smem_u32(raw));
   uint64_t* bars = reinterpret_cast<uint64_t*>(shared + Sh::kBars);
+  __shared__ int64_t s_scan[kPromptThreads / 32];
+  __shared__ PromptItem s_item;
+  __shared__ int s_unit;
   pdl_wait();
-  // Items in order: requests, heads, row blocks. Each warp walks them for itself, 32 requests at a time (a lane each);
-  // all find the same ones.
+  // The items, requests outermost, then heads, then row blocks (the last rows, which see the most keys under a causal mask, first),
+  // form one line of steps that the CTAs cut into equal shares. Total and place by a block scan over the requests.
   const int heads = a.kv.heads;
-  PromptItem it;
-  int window = -32;                          // first request of the window
-  int64_t first = 0, window_items = 0;       // items before the window, and in it
-  int64_t lane_items = 0, lane_before = 0;   // of this lane's request
-  AttnRequest lane_rq = {};
-  auto next_item = [&](int64_t index) {
-    while (index >= first + window_items) {
-      window += 32;
-      if (window >= a.B) return false;
-      first += window_items;
-      lane_items = 0;
-      if (window + lane < a.B) {
-        lane_rq = attn_request<8>(a, window + lane, nullptr, false);
-        const int64_t rows = (int64_t)lane_rq.qlen * a.group;
-        if (rows > a.split_rows) lane_items = (rows + kPromptRows - 1) / kPromptRows * heads;
-      }
-      int64_t incl = lane_items;
+  int32_t* desc = a.desc + (int64_t)blockIdx.x * kAttnDescInts;
+  const int per = (a.B + kPromptThreads - 1) / kPromptThreads;
+  const int rb0 = min(a.B, tid * per), rb1 = min(a.B, rb0 + per);
+  int64_t mine = 0;
+  for (int b = rb0; b < rb1; ++b) mine += prompt_work(a, attn_request<8>(a, b, nullptr, false)) * heads;
+  int64_t incl = mine;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += y;
-      }
-      lane_before = incl - lane_items;
-      window_items = __shfl_sync(0xffffffffu, incl, 31);
-    }
-    const int64_t at = index - first;
-    const int src = __ffs(__ballot_sync(0xffffffffu, at >= lane_before && at < lane_before + lane_items)) - 1;
-    it.b = window + src;
-    it.rq.q0 = __shfl_sync(0xffffffffu, lane_rq.q0, src);
-    it.rq.qlen = __shfl_sync(0xffffffffu, lane_rq.qlen, src);
-    it.rq.n = __shfl_sync(0xffffffffu, lane_rq.n, src);
-    const int blocks = (int)(__shfl_sync(0xffffffffu, lane_items, src) / heads);
-    const int rest = (int)(at - __shfl_sync(0xffffffffu, lane_before, src));
-    it.head = rest / blocks;
-    // the longest first: under a causal mask the last rows see the most keys
-    it.row0 = (blocks - 1 - rest % blocks) * kPromptRows;
-    it.rows = min(kPromptRows, it.rq.qlen * a.group - it.row0);
-    const int last = (it.row0 + it.rows - 1) / a.group;
-    const int seen = a.causal ? min(it.rq.n, max(0, it.rq.n - it.rq.qlen + last + 1)) : it.rq.n;
-    it.steps = (seen + kPromptKeys - 1) / kPromptKeys;
-    return true;
-  };
-  if (!next_item(blockIdx.x)) {  // nothing for this CTA
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += y;
+  }
+  if (lane == 31) s_scan[warp] = incl;
+  __syncthreads();
+  int64_t total = 0, before = incl - mine;
+  for (int w = 0; w < kPromptThreads / 32; ++w) {
+    if (w < warp) before += s_scan[w];
+    total += s_scan[w];
+  }
+  const int64_t share = max((total + gridDim.x - 1) / gridDim.x, (int64_t)kPromptMinShare);
+  int64_t at = (int64_t)blockIdx.x * share;
+  const int64_t end = min(at + share, total);
+  if (at >= end) {  // nothing for this CTA
+    if (tid == 0) desc[0] = 0;
     pdl_launch_dependents();
     return;
   }
+  if (at >= before && at < before + mine) {
+    int64_t rem = at - before;
+    PromptItem x;
+    for (x.b = rb0;; ++x.b) {
+      x.rq = attn_request<8>(a, x.b, nullptr, false);
+      const int64_t w = prompt_work(a, x.rq);
+      if (rem < w * heads) {
+        x.head = (int)(rem / w);
+        rem %= w;
+        break;
+      }
+      rem -= w * heads;
+    }
+    for (x.block = prompt_blocks(a, x.rq) - 1;; --x.block) {
+      const int w = max(1, prompt_steps(a, x.rq, x.block)) + kPromptLead;
+      if (rem < w) break;
+      rem -= w;
+    }
+    s_item = x;
+    s_unit = (int)rem - kPromptLead;  // below 0: the start's cost
+  }
+  __syncthreads();
+  PromptItem it = s_item;
+  int unit = s_unit;
+  int32_t parts = 0, part_q0 = 0, part_qlen = 0, part_row = 0, part_head = 0;  // of an item that goes on in the next CTA
+  // The next stretch of this share, into `it`; every warp walks the share for itself.
+  auto next_item = [&]() {
+    if (at >= end) return false;
+    int steps = prompt_steps(a, it.rq, it.block), units = max(1, steps);
+    if (unit == units) {
+      unit = -kPromptLead;
+      if (--it.block < 0) {
+        if (++it.head == heads) {
+          it.head = 0;
+          do it.rq = attn_request<8>(a, ++it.b, nullptr, false); while (prompt_blocks(a, it.rq) == 0);  // at < end: there is one
+        }
+        it.block = prompt_blocks(a, it.rq) - 1;
+      }
+      steps = prompt_steps(a, it.rq, it.block);
+      units = max(1, steps);
+    }
+    const int lead = (int)min((int64_t)max(-unit, 0), end - at);
+    at += lead;
+    unit += lead;
+    if (at == end) return false;
+    const int take = (int)min((int64_t)(units - unit), end - at);
+    it.row0 = it.block * kPromptRows;
+    it.rows = min(kPromptRows, it.rq.qlen * a.group - it.row0);
+    it.u0 = min(unit, steps);
+    it.u1 = min(unit + take, steps);
+    it.starts = unit == 0;
+    it.ends = unit + take == units;
+    if (it.starts && !it.ends) {
+      parts = (int)((at + units - 1) / share - blockIdx.x) + 1;
+      part_q0 = it.rq.q0;
+      part_qlen = it.rq.qlen;
+      part_row = it.row0;
+      part_head = it.head;
+    }
+    at += take;
+    unit += take;
+    return true;
+  };
 
   if (tid == 0) {
     s_stop = 0;
@@ -315,10 +383,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
     uint32_t s_phase = 0, o_phase = 0, p_phase = 0, q_phase = 0;
     uint32_t done = 0;  // steps so far, over all items, this tile's rows at work or not
     bool go = true;
-    for (int64_t item = blockIdx.x; go && next_item(item); item += gridDim.x) {
+    while (go && next_item()) {
       if (tile * 128 >= it.rows) {
         // No rows: the tile still takes and gives back each stage, or it would meet the next item's barriers phases early.
-        for (int j = 0; issuer && j < it.steps; ++j) {
+        for (int j = 0; issuer && j < it.u1 - it.u0; ++j) {
           const int stage = (done + j) & 1;
           const uint32_t parity = ((done + j) >> 1) & 1;
           if (!wait(kKFull + stage, parity)) break;
@@ -327,7 +395,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
           mbar_arrive(&bars[kVEmpty + stage]);
         }
         __syncwarp();
-        done += it.steps;
+        done += it.u1 - it.u0;
         continue;
       }
       const int row = it.row0 + tile * 128 + r;
@@ -336,7 +404,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
       const int sub = row - tok * a.group;
       const int lim = a.causal ? min(it.rq.n, max(0, it.rq.n - it.rq.qlen + tok + 1)) : it.rq.n;
       float qsum = 0.0f, unscale = 1.0f;
-      if (it.steps > 0) {
+      if (it.u1 > it.u0) {
         // The row as fp16, a bf16 one scaled by a power of two to a largest element of 2^11 to 2^12 (as in attn_int4.cuh).
         const uint16_t* src = static_cast<const uint16_t*>(a.q) + (int64_t)(it.rq.q0 + tok) * a.qsn +
                               ((int64_t)it.head * a.group + (here ? sub : 0)) * a.qsh;
@@ -377,7 +445,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
       }
       float m = -INFINITY, l = 0.0f;
       float2 r2 = both(0.0f);
-      for (int j = 0; go && j < it.steps; ++j, ++done) {
+      for (int j = it.u0; go && j < it.u1; ++j, ++done) {
         const int buf = done & 3;
         const uint32_t parity = (done >> 2) & 1;
         go = wait(kSFull + tile, s_phase) && wait(kKeyFac + buf, parity) && wait(kValueFac + buf, parity);
@@ -439,7 +507,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
             const float was = m;
             m = up ? cand : m;
             const float factor = was == m || was == -INFINITY ? 1.0f : ex2(was - m);  // before its first key the row of O is zeros
-            if (j > 0) {
+            if (j > it.u0) {
 #pragma unroll 1
               for (int d = 0; d < D / 32; ++d) {
                 uint32_t o[32];
@@ -484,15 +552,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
         tmem_fence_before();
         mbar_arrive(&bars[kPFull + tile]);
         if (issuer && wait(kPFull + tile, p_phase)) {
-          issue_values(done, j > 0);
-          if (j + 1 < it.steps) issue_scores(done + 1);
+          issue_values(done, j > it.u0);
+          if (j + 1 < it.u1) issue_scores(done + 1);
           else umma_commit(&bars[kOFull + tile]);
         }
         __syncwarp();
         p_phase ^= 1;
       }
       if (!go) break;
-      if (it.steps > 0) {
+      if (it.u1 > it.u0) {
         go = wait(kOFull + tile, o_phase);
         o_phase ^= 1;
         if (!__all_sync(0xffffffffu, go)) {
@@ -501,28 +569,33 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
         }
         tmem_fence_after();
       }
-      const float inv = l != 0.0f ? 1.0f / l : 0.0f, rest = r2.x + r2.y;
+      const bool whole = it.starts && it.ends;
+      const float inv = whole ? (l != 0.0f ? 1.0f / l : 0.0f) : 1.0f, rest = r2.x + r2.y;
+      float* part = a.part + ((int64_t)blockIdx.x * 2 + (it.starts && !it.ends ? 1 : 0)) * attn_part_floats(D, kPromptRows);
+      float* part_row_at = part + (tile * 128 + r) * D;
       uint16_t* dst = static_cast<uint16_t*>(a.out) + (int64_t)(it.rq.q0 + tok) * a.osn +
                       ((int64_t)it.head * a.group + sub) * a.osh;
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
-        if (it.steps > 0) {
-          tmem_ld32(o, o_addr + c * 32);
-        }
+        if (it.u1 > it.u0) tmem_ld32(o, o_addr + c * 32);
 #pragma unroll
         for (int i = 0; i < 32; i += 8) {
           float f[8];
 #pragma unroll
           for (int x = 0; x < 8; ++x) f[x] = l != 0.0f ? (__uint_as_float(o[i + (x < 4 ? 2 * x : 2 * x - 7)]) + rest) * inv : 0.0f;
-          if (here) {
+          if (here && !whole) {
+            *reinterpret_cast<float4*>(part_row_at + c * 32 + i) = make_float4(f[0], f[1], f[2], f[3]);
+            *reinterpret_cast<float4*>(part_row_at + c * 32 + i + 4) = make_float4(f[4], f[5], f[6], f[7]);
+          } else if (here) {
             if (a.o_vec) kv_store8<true>(dst + c * 32 + i, pack8<T>(f));
             else kv_store8<false>(dst + c * 32 + i, pack8<T>(f));
           }
         }
       }
       tmem_fence_before();
-      if (here && a.lse != nullptr)
+      if (here && !whole) *reinterpret_cast<float2*>(part + kPromptRows * D + 2 * (tile * 128 + r)) = make_float2(m, l);
+      if (here && whole && a.lse != nullptr)
         a.lse[(int64_t)(it.rq.q0 + tok) * heads * a.group + (int64_t)it.head * a.group + sub] =
             l != 0.0f ? m + __log2f(l) : -INFINITY;
     }
@@ -542,12 +615,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
     constexpr int kVecs = D / 32;  // 16-byte vectors of a row's codes
     uint32_t done = 0;             // steps unpacked so far, over all items
     bool go = true;
-    for (int64_t item = blockIdx.x; go && next_item(item); item += gridDim.x) {
+    while (go && next_item()) {
       const int32_t* table = a.block_tables + (int64_t)it.b * a.table_stride;
       // The page of this thread's key in step j, -1 past the cache's end and for a bad one.
       auto find = [&](int j) {
         const int tok = j * kPromptKeys + r;
-        if (j >= it.steps || tok >= it.rq.n) return -1;
+        if (j >= it.u1 || tok >= it.rq.n) return -1;
         const int page = table[a.page_shift >= 0 ? tok >> a.page_shift : tok / (int)a.kv.page_size];
         if (page >= 0 && page < a.kv.num_pages) return page;
         if (!values) flag_status(a.status, MAS_STATUS_KV_SLOT_OUT_OF_RANGE);
@@ -574,9 +647,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
       // The codes of the next step and the page of the one after it are on their way while a step is unpacked.
       uint32_t w[D / 8];
       uint2 pair;
-      load(0, find(0), w, pair);
-      int page = find(1);
-      for (int j = 0; j < it.steps; ++j, ++done) {
+      load(it.u0, find(it.u0), w, pair);
+      int page = find(it.u0 + 1);
+      for (int j = it.u0; j < it.u1; ++j, ++done) {
         const int stage = done & 1;
         uint32_t w_next[D / 8];
         uint2 pair_next;
@@ -626,6 +699,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
   __syncwarp();
   tmem_fence_before();
   __syncthreads();
+  if (tid == 0) {
+    desc[0] = parts;
+    desc[1] = part_q0;
+    desc[2] = part_qlen;
+    desc[3] = part_row;
+    desc[4] = part_head;
+  }
   if (warp == 0) {
     tmem_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));

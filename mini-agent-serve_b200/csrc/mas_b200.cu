@@ -720,7 +720,8 @@ int64_t attn_ctas(const DeviceState& st, int NT) {
 int64_t attn_part_bytes(const DeviceState& st, int64_t head_size) {
   int64_t most = 0;
   for (int nt = 1; nt <= 2; ++nt)
-    most = std::max(most, attn_ctas(st, nt) * 2 * kAttnMaxHeads * attn_part_floats((int)head_size, nt));
+    most = std::max(most, attn_ctas(st, nt) * 2 * kAttnMaxHeads * attn_part_floats((int)head_size, 8 * nt));
+  most = std::max(most, (int64_t)st.sm_count * 2 * attn_part_floats((int)head_size, kPromptRows));
   return most * (int64_t)sizeof(float);
 }
 int64_t attn_workspace_bytes(const DeviceState& st, int64_t head_size) {
@@ -742,7 +743,7 @@ int launch_attn_int4(AttnInt4Args a, DeviceState* st, void* stream, int enable_p
   const int rc = launch(attn_int4_kernel<T, D, NT>, dim3(grid), dim3(kAttnThreads), AttnInt4Shape<D, NT>::kSmem, stream,
                         enable_pdl, a);
   if (rc != MAS_OK || !split) return rc;
-  return launch(attn_int4_join_kernel<T, D, NT>, dim3(grid, a.cta_heads * 8 * NT / kAttnWarps), dim3(kAttnThreads), 0,
+  return launch(attn_int4_join_kernel<T, D, 8 * NT>, dim3(grid, a.cta_heads * 8 * NT / kAttnWarps), dim3(kAttnThreads), 0,
                 stream, enable_pdl, a);
 }
 
@@ -759,11 +760,15 @@ int run_attn_int4(AttnInt4Args a, DeviceState* st, void* stream, int enable_pdl)
   const int64_t min_rows = env_min >= 0 ? env_min : (int64_t)kPromptRowsPerSm * st->sm_count;
   if (a.cum_q != nullptr && a.T * a.group > kAttnSplitRows && a.T * a.group * a.kv.heads >= min_rows) {
     a.split_rows = kAttnSplitRows;
-    const int64_t items = (ceil_div(a.T * a.group, kPromptRows) + a.B) * a.kv.heads;
-    const unsigned grid = (unsigned)std::min<int64_t>(items, st->sm_count);
+    const unsigned grid = (unsigned)st->sm_count;
     const int rc = launch(attn_int4_prompt_kernel<T, D>, dim3(grid), dim3(kPromptThreads), PromptShape<D>::kSmem, stream,
                           enable_pdl, a, st->fault);
     if (rc != MAS_OK) return rc;
+    AttnInt4Args join = a;
+    join.cta_heads = 1;
+    const int rj = launch(attn_int4_join_kernel<T, D, kPromptRows>, dim3(grid, kPromptRows / kAttnWarps), dim3(kAttnThreads), 0,
+                          stream, enable_pdl, join);
+    if (rj != MAS_OK) return rj;
     if (rows > kAttnSplitRows) rows = a.group;  // prompts in the mean: what is left are decode rows
   }
   if (rows <= 8) return launch_attn_int4<T, D, 1>(a, st, stream, enable_pdl);
