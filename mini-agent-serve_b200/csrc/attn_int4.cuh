@@ -847,17 +847,16 @@ __global__ void __launch_bounds__(kAttnThreads, AttnInt4Shape<D, NT>::kCtasPerSm
   pdl_launch_dependents();
 }
 
-// Joins the parts of the tiles that were split: CTA (c, y) takes four (head, row) pairs of the tile that the
+// Joins the parts of the tiles that were split: CTAs (c, y) take the (head, row) pairs of the tile that the
 // main kernel's CTA c started, a warp each, in the order of the parts.
 template <typename T, int D, int kRows>
 __global__ void __launch_bounds__(kAttnThreads) attn_int4_join_kernel(const AttnInt4Args a) {
   pdl_wait();
   const int lane = threadIdx.x & 31;
-  const int hr = blockIdx.y * kAttnWarps + (threadIdx.x >> 5);
-  const int which = hr / kRows, r = hr % kRows;
   const int32_t* desc = a.desc + (int64_t)blockIdx.x * kAttnDescInts;
   const int parts = desc[0];
-  if (parts > 0) {
+  for (int hr = blockIdx.y * kAttnWarps + (threadIdx.x >> 5); parts > 0 && hr < a.cta_heads * kRows; hr += gridDim.y * kAttnWarps) {
+    const int which = hr / kRows, r = hr % kRows;
     const int q0 = desc[1], row = desc[3] + r, head = desc[4] + which;
     if (row < desc[2] * a.group) {
       constexpr int kPer = D / 32;

@@ -8,9 +8,9 @@
 // (ks, kb the key's scale and minimum + 8 scales, times the softmax scale and log2 e). M is one reference for all: the row's
 // largest log2 of a weight p sv, moved when one passes it by 8.
 //
-// Measured: 911 and 1511 new tokens of 6 K (96/8 heads of 128) take 1385 us against a floor of 393 (products). What bounds it is the
-// softmax warps, two a scheduler, which issue in 36 % of the cycles: without their arithmetic 749 us, without exponentials 1294,
-// without factor loads 1213. Sixteen softmax warps of half a row a thread took 1798 (104 registers spill), two S buffers of 64 keys a
+// Measured: 911 and 1511 new tokens of 6 K (96/8 heads of 128) take 1292 us against a floor of 393
+// (products); 1385 with the items dealt to the SMs whole. What bounds it is the softmax warps, two a scheduler, which issue in 36 % of the cycles: of the 1385, their arithmetic is 636 us, exponentials alone 91,
+// factor loads 172. Sixteen softmax warps of half a row a thread took 1798 (104 registers spill), two S buffers of 64 keys a
 // tile 15 % more than this. Keys and values rounded to bf16 on the way in, two instructions less a (row, key), took 924, but were
 // 0.0051 of the result off where this is 0.0017.
 //
@@ -42,10 +42,13 @@ constexpr int kPromptThreads = 512;
 constexpr int kPromptSoftmaxRegs = 168, kPromptUnpackRegs = 88;
 constexpr int kPromptRows = 256;  // rows of a CTA's item
 constexpr int kPromptKeys = 128;  // keys of a step
-// Requests with more rows a kv head go to this kernel, in calls with enough rows to give the SMs work without cutting contexts.
-// 16 requests over 4 K tokens (96/8 heads), this kernel against tiles of 16 rows: 72 rows 144 and 115 us, 96 rows 146 and 135,
-// 132 rows (114 a SM in all) 188 and 192, 192 rows (166 a SM) 192 and 248.
-constexpr int kAttnSplitRows = 96, kPromptRowsPerSm = 160;
+// Requests with more rows a kv head go to this kernel, in calls with enough rows (over all heads) an SM to pay for the launches.
+// 96/8 heads of 128, this kernel against tiles of 16 rows. 16 requests over 4 K tokens: 72 rows a kv head 131 and 116 us, 96 rows 151
+// and 136, 132 rows 170 and 192, 288 rows 275 and 359. Rows an SM: 28 (4 requests of 132 rows, 4 K) 69 and 64 us, 51 (of 240) 80 and
+// 89; over 600 tokens 111 an SM take 70 and 54, over 15 K 12 an SM 84 and 85.
+// (The least is above the break-even: a call with many rows and no such request pays 7 us for nothing.)
+constexpr int kAttnSplitRows = 96, kPromptRowsPerSm = 64;
+constexpr int kPromptJoinCtas = 16;  // a CTA's item in the joining kernel (64 cost an empty launch 10 us more)
 
 template <int D>
 struct PromptShape {
@@ -167,8 +170,9 @@ __device__ __forceinline__ void unpack_row(uint32_t base, int row, const uint32_
   }
 }
 
-// What starting on an item costs (its queries, the first loads' latency), in steps, and the fewest steps of a share.
-constexpr int kPromptLead = 2, kPromptMinShare = 8;
+// What starting on an item costs (its queries, the first loads' latency), in steps (0, 1, 4 instead: 1295, 1295, 1288 us where 2 takes
+// 1292), and the least share: one step past that (132 rows over 600 tokens: 47 us, 53 with 4, 70 with 8).
+constexpr int kPromptLead = 2, kPromptMinShare = 3;
 
 // A stretch of the line of work: steps u0 .. u1 of an item, 256 rows of one kv head of one request.
 struct PromptItem {

@@ -755,10 +755,10 @@ int run_attn_int4(AttnInt4Args a, DeviceState* st, void* stream, int enable_pdl)
   int64_t rows = ceil_div(a.T, a.B) * a.group;
   a.split_rows = INT32_MAX;
   // The lengths are the device's: where some request may have more than kAttnSplitRows rows, the prompt kernel is launched
-  // for those and this one leaves them out; both may find nothing. The prompt kernel does not cut contexts, so it needs items: 160 rows an SM.
+  // for those and this one leaves them out; both may find nothing (no more tokens than requests are taken for decode rows). Both rules' figures stand at the constants.
   static const int env_min = env_int("MAS_ATTN_PROMPT_MIN_ROWS", -1);
   const int64_t min_rows = env_min >= 0 ? env_min : (int64_t)kPromptRowsPerSm * st->sm_count;
-  if (a.cum_q != nullptr && a.T * a.group > kAttnSplitRows && a.T * a.group * a.kv.heads >= min_rows) {
+  if (a.cum_q != nullptr && a.T > a.B && a.T * a.group > kAttnSplitRows && a.T * a.group * a.kv.heads >= min_rows) {
     a.split_rows = kAttnSplitRows;
     const unsigned grid = (unsigned)st->sm_count;
     const int rc = launch(attn_int4_prompt_kernel<T, D>, dim3(grid), dim3(kPromptThreads), PromptShape<D>::kSmem, stream,
@@ -766,8 +766,8 @@ int run_attn_int4(AttnInt4Args a, DeviceState* st, void* stream, int enable_pdl)
     if (rc != MAS_OK) return rc;
     AttnInt4Args join = a;
     join.cta_heads = 1;
-    const int rj = launch(attn_int4_join_kernel<T, D, kPromptRows>, dim3(grid, kPromptRows / kAttnWarps), dim3(kAttnThreads), 0,
-                          stream, enable_pdl, join);
+    const int rj = launch(attn_int4_join_kernel<T, D, kPromptRows>, dim3(grid, kPromptJoinCtas), dim3(kAttnThreads), 0, stream,
+                          enable_pdl, join);
     if (rj != MAS_OK) return rj;
     if (rows > kAttnSplitRows) rows = a.group;  // prompts in the mean: what is left are decode rows
   }

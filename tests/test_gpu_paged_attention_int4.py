@@ -56,11 +56,11 @@ def _make(seed, lens, hkv, d, page_size, layout, poison=True, v_scale=1.0):
     return (codes[0], codes[1], pairs), table
 
 
-def _takes_prompt_kernel(tokens: int, hq: int, rows: int) -> bool:
+def _takes_prompt_kernel(tokens: int, requests: int, hq: int, rows: int) -> bool:
     """The library's choice for a request with that many rows a kv head."""
     least = os.environ.get("MAS_ATTN_PROMPT_MIN_ROWS")
-    least = int(least) if least else 160 * torch.cuda.get_device_properties(0).multi_processor_count
-    return rows > 96 and tokens * hq >= least
+    least = int(least) if least else 64 * torch.cuda.get_device_properties(0).multi_processor_count
+    return tokens > requests and rows > 96 and tokens * hq >= least
 
 
 def _bound(q, cache, layout, table, lens, cum, scale, causal, dtype):
@@ -77,7 +77,7 @@ def _bound(q, cache, layout, table, lens, cum, scale, causal, dtype):
         pr = cache[2].double()[pages, :, entries]                       # [n, h, 4]
         # what the codes are centred on: the tensor-core kernel's rows, the other's for fp16 and for bf16
         z = 0.0 if dtype == BF else 7.5
-        if _takes_prompt_kernel(T, hq, (cum[b + 1] - cum[b]) * (hq // h)):
+        if _takes_prompt_kernel(T, len(lens), hq, (cum[b + 1] - cum[b]) * (hq // h)):
             z = 8.0
         code = (v - pr[..., 3, None]) / pr[..., 2, None]
         for i in range(cum[b], cum[b + 1]):
