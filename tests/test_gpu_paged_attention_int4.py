@@ -192,6 +192,12 @@ def test_prompt_rows_of_odd_pages_and_scales(cuda, causal):
     _run(66, [500], [40], 6, 2, 128, BF, causal=causal, v_scale=1e30)
 
 
+@pytest.mark.parametrize("causal", [True, False])
+def test_prompt_rows_of_a_long_context(cuda, causal):
+    """One item of two tiles and one of a few rows, both cut into many parts."""
+    _run(78, [6000, 5000], [40, 70], 4, 1, 128, BF, causal=causal)
+
+
 @pytest.mark.parametrize("dtype", [BF, FP])
 def test_prompt_rows_beside_decode_rows(cuda, dtype):
     """A mixed step at the 123B-class head counts, large enough for the prompt kernel by itself."""
