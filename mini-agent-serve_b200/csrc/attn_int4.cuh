@@ -47,6 +47,9 @@ constexpr int kAttnMaxHeads = 2;  // kv heads a CTA takes at once
 // with 0, 271 with 2, 255 with 4, 256 with 6 (before the products were all fp16).
 constexpr int kAttnLead = 4;
 
+// How far a logit (log2), and so a p, may lie past its row's reference before the reference moves.
+constexpr float kAttnFarLogit = 12.0f, kAttnFarP = 4096.0f;
+
 struct AttnInt4Args {
   const void* q;
   void* out;
@@ -565,14 +568,14 @@ __global__ void __launch_bounds__(kAttnThreads, AttnInt4Shape<D, NT>::kCtasPerSm
         apart = __any_sync(0xffffffffu, odd != 0.0f);
       }
 
-      float2 l_new[NT], r_new[NT];
+      float2 p_sum[NT], r_new[NT];
       uint32_t wh[kPass][NT][2];
       uint32_t top;  // the largest weights, a NaN before all (0 * infinity, of a logit far past the reference, is one)
       auto weigh = [&](auto masked) {
         top = 0;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          l_new[nt] = l[nt];
+          p_sum[nt] = both(0.0f);
           r_new[nt] = r[nt];
 #pragma unroll
           for (int x = 0; x < kPass; ++x)
@@ -589,7 +592,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnInt4Shape<D, NT>::kCtasPerSm
                 vmh.x = sv.x == -INFINITY ? 0.0f : vmh.x;
                 vmh.y = sv.y == -INFINITY ? 0.0f : vmh.y;
               }
-              l_new[nt] = add2_f32(l_new[nt], p);
+              p_sum[nt] = add2_f32(p_sum[nt], p);
               r_new[nt] = fma2_f32(p, vmh, r_new[nt]);
               wh[x][nt][half] = Elem<__half>::from_f2(w.x, w.y);
               top = max_nan_half2(top, wh[x][nt][half]);
@@ -599,10 +602,14 @@ __global__ void __launch_bounds__(kAttnThreads, AttnInt4Shape<D, NT>::kCtasPerSm
       weigh(std::false_type{});
       if (apart) weigh(std::true_type{});
       const bool first = i == 0 && p0 == 0;
-      // The references move only when a weight passes 1024 (fp32 sums and fp16 weights have that much room), and with
-      // the first step: the accumulators are then rescaled, which most steps need not do. A half above 1024
-      // (0x6400), an infinity or a NaN carries into its sign bit.
-      if (first || __any_sync(0xffffffffu, (top + 0x1bff1bffu) & 0x80008000u)) {
+      // The references move only when a weight passes 1024 (fp32 sums and fp16 weights have that much room), when a p passes
+      // 2^12 (the weights of values of next to no spread never grow, but their minima enter with p alone: r stays finite for
+      // values up to 2^90 and more tokens than fit), and with the first step: the accumulators are then rescaled, which most
+      // steps need not do. A half above 1024 (0x6400), an infinity or a NaN carries into its sign bit.
+      bool far = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) far |= fmaxf(p_sum[nt].x, p_sum[nt].y) > kAttnFarP * (2 * kPass);
+      if (first || __any_sync(0xffffffffu, ((top + 0x1bff1bffu) & 0x80008000u) || far)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float hi[2] = {-INFINITY, -INFINITY}, hw[2] = {-INFINITY, -INFINITY}, seen[2] = {l[nt].x, l[nt].y};
@@ -634,7 +641,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnInt4Shape<D, NT>::kCtasPerSm
             const float old = seen[c] == 0.0f ? -INFINITY : -nr[c];
             const float was = old - __log2f(ws[c]);
             fl[c] = fo[c] = 1.0f;
-            if (!(hw[c] > was + 10.0f || hi[c] > old + 100.0f)) continue;
+            if (!(hw[c] > was + 10.0f || hi[c] > old + kAttnFarLogit)) continue;
             const float now = fmaxf(old, hi[c]);
             const float room = floorf(now - fmaxf(was, hw[c]));
             const float nws = now == -INFINITY ? 1.0f : __uint_as_float((uint32_t)(fminf(fmaxf(room, -126.0f), 127.0f) + 127.0f) << 23);
@@ -661,7 +668,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnInt4Shape<D, NT>::kCtasPerSm
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        l[nt] = l_new[nt];
+        l[nt] = add2_f32(l[nt], p_sum[nt]);
         r[nt] = r_new[nt];
       }
 #pragma unroll

@@ -1,0 +1,165 @@
+"""Attention over the 4-bit cache at the ends of its ranges: value and key rows of very unlike scales in one cache, constant
+rows, logits far apart, small queries under a large scale.
+
+All requests of a call have the same lengths here, so the 64-bit form is a few dense products. Tolerance, per element, with p
+normalised over n keys, w = p s the weight that a key's code carries, z what the codes are centred on (0: bf16 results, 7.5: fp16
+ones, 8: the prompt kernel):
+- w is rounded to fp16: 2^-11 of it (twice in the prompt kernel, where the reference may move between the halves of a step), and,
+  below fp16's normal numbers, half of their step 2^-24 or all of w. The largest weight since its reference last moved lies in 1/2 to
+  1024: the step is at most 2^-23 of the row's largest w. In the prompt kernel the reference follows the largest of
+  max(s, |m + 8 s| 2^-60, 2^-96) p, up to a spread of 2^10 within a step, from below 2^8: 2^-14 of the largest such product;
+- sums over n keys in fp32, by steps of 16 in the matrix unit: u = 2^-22 (n / 16 + 32) of the terms' sizes, at most (15 + z) w and
+  p (|m| + z s);
+- a logit is off by delta = sm_scale 2^-23 (D / 8 + 6) max_t (143 s_t + |m_t|) sum |q| (of the keys): D / 16 steps of the matrix unit,
+  two roundings each, and six more operations, on terms of at most 15 s |q|. It enters as 2 delta (sum p |v| + |o|);
+- a p below 2^-126 of its reference, which is at most 2^20 from the largest, is zero: 2^-100 of the largest |v|, n times; a
+  weight below all the types' ranges: 16 steps of 2^-126;
+- the result is rounded: eps_T / 2 |o|, or half a step of fp16's least numbers.
+"""
+from __future__ import annotations
+
+import math
+import os
+
+import pytest
+import torch
+
+import mas_b200
+
+pytestmark = pytest.mark.gpu
+
+BF, FP = torch.bfloat16, torch.float16
+LEAST = 2.0 ** -126  # a constant row's scale
+
+
+def _prompt_kernel(tokens: int, requests: int, hq: int, rows: int) -> bool:
+    """The library's choice for requests with that many rows a kv head."""
+    least = os.environ.get("MAS_ATTN_PROMPT_MIN_ROWS")
+    least = int(least) if least else 64 * torch.cuda.get_device_properties(0).multi_processor_count
+    return tokens > requests and rows > 96 and tokens * hq >= least
+
+
+def _cache(codes, kp, vp, page_size, layout):
+    """A paged cache with the given rows, pages in a shuffled order. codes: two [B, n, h, D] of 0..15; kp, vp: [B, n, h, 2]."""
+    B, n, h, d = codes[0].shape
+    blocks = -(-n // page_size)
+    table = torch.randperm(B * blocks, device="cuda").to(torch.int32).view(B, blocks)
+    cache = mas_b200.empty_paged_kv_cache_int4(B * blocks, page_size, h, d, layout)
+    cache[2].fill_(math.nan)
+    tok = torch.arange(n, device="cuda")
+    pages, entries = table[:, tok // page_size].long(), (tok % page_size).expand(B, n)
+    for t, c in zip(cache, codes):
+        packed = (c[..., 0::2] | (c[..., 1::2] << 4)).to(torch.uint8)
+        if layout == "NHD":
+            t[pages, entries] = packed
+        else:
+            t[pages, :, entries] = packed
+    cache[2][pages, :, entries] = torch.cat([kp, vp], -1)
+    return cache, table
+
+
+def _codes(g, shape):
+    return torch.randint(0, 16, shape, generator=g, device="cuda")
+
+
+def _expect(q, codes, kp, vp, ql, scale, causal, prompt):
+    """(out, tol, lse, ltol): [B * ql, hq, D], lse [B * ql, hq], in 64 bits."""
+    B, n, h, d = codes[0].shape
+    hq = q.shape[1]
+    dtype = q.dtype
+    kc, vc, kp, vp = codes[0].double(), codes[1].double(), kp.double(), vp.double()
+    k, v = (c * p[..., :1] + p[..., 1:] for c, p in ((kc, kp), (vc, vp)))
+    qd = q.double().view(B, ql, h, hq // h, d)
+    s = torch.einsum("bqhgd,bnhd->bhgqn", qd, k) * scale
+    if causal:
+        seen = torch.arange(n, device="cuda") <= torch.arange(n - ql, n, device="cuda")[:, None]
+        s = s.masked_fill(~seen, -math.inf)
+    lse = torch.logsumexp(s, -1)
+    p = torch.where(lse[..., None].isinf(), 0.0, (s - lse[..., None]).exp())
+    mix = lambda w, x: torch.einsum("bhgqn,bnhd->bhgqd", w, x)  # noqa: E731
+    out = mix(p, v)
+    z = 8.0 if prompt else 7.5 if dtype == FP else 0.0
+    col = lambda x: x.transpose(1, 2)[:, :, None, None]  # noqa: E731  [b, n, h] -> [b, h, 1, 1, n]
+    sv, mv = col(vp[..., 0]), col(vp[..., 1])
+    w = p * sv
+    if prompt:
+        reach = torch.maximum(torch.maximum(sv, (mv + 8 * sv).abs() * 2.0 ** -60), torch.tensor(2.0 ** -96, device="cuda"))
+        least = 2.0 ** -14 * (p * reach).amax(-1, keepdim=True)
+    else:
+        least = 2.0 ** -23 * w.amax(-1, keepdim=True)
+    err = mix((2.0 ** -10 if prompt else 2.0 ** -11) * w + torch.minimum(w, least), (vc - z).abs())
+    u = 2.0 ** -22 * (n / 16 + 32)
+    err = err + u * (w * (15 + z) + p * (mv.abs() + z * sv)).sum(-1, keepdim=True)
+    keys = (143 * kp[..., 0] + kp[..., 1].abs()).amax(1)  # [b, h]
+    delta = 2.0 ** -23 * (d / 8 + 6) * abs(scale) * keys[:, :, None, None] * qd.abs().sum(-1).permute(0, 2, 3, 1)
+    err = err + 2 * delta[..., None] * (mix(p, v.abs()) + out.abs())
+    largest = torch.where(s.isinf(), 0.0, col(v.abs().amax(-1))).amax(-1, keepdim=True)
+    err = err + n * 2.0 ** -100 * largest + 16 * LEAST
+    err = err + torch.finfo(dtype).eps / 2 * torch.maximum(out.abs(), torch.tensor(torch.finfo(dtype).tiny, device="cuda"))
+    lse2 = lse / math.log(2)
+    ltol = delta * 1.4427 + 2.0 ** -20 * (1 + lse2.abs()) + u
+    back = lambda x: x.permute(0, 3, 1, 2, *range(4, x.dim())).reshape(B * ql, hq, *x.shape[4:])  # noqa: E731
+    return back(out), back(err), back(lse2), back(ltol)
+
+
+def _check(q, codes, kp, vp, ql, dtype, scale=None, causal=True, layout="NHD", page_size=16):
+    B, n, h, d = codes[0].shape
+    q = q.to(dtype)
+    scale = d ** -0.5 if scale is None else scale
+    cache, table = _cache(codes, kp, vp, page_size, layout)
+    lens = torch.full((B,), n, dtype=torch.int32, device="cuda")
+    cum = torch.arange(B + 1, dtype=torch.int32, device="cuda") * ql
+    mas_b200.read_status()
+    got, glse = mas_b200.paged_attention_int4(q, cache, table, lens, cum, sm_scale=scale, causal=causal, kv_layout=layout,
+                                              return_lse=True)
+    assert mas_b200.read_status() == 0
+    prompt = _prompt_kernel(B * ql, B, q.shape[1], ql * q.shape[1] // h)
+    want, tol, lse, ltol = _expect(q, codes, kp, vp, ql, scale, causal, prompt)
+    top = torch.finfo(dtype).max
+    assert want.abs().max() < top
+    bad = ~((got.double() - want).abs() <= tol)
+    assert not bad.any(), (int(bad.sum()), bad.nonzero()[0].tolist(), got[bad][0].item(), want[bad][0].item(), tol[bad][0].item())
+    hidden = lse.isinf()
+    assert torch.equal(glse.isinf(), hidden) and (got[hidden] == 0).all()
+    lerr = torch.where(hidden, 0.0, (glse.double() - torch.where(hidden, 0.0, lse)).abs())
+    assert (lerr <= ltol).all(), lerr.max()
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _pairs(s, m):
+    return torch.stack([s, m], -1).to(BF)
+
+
+def _plain_pairs(g, shape, scale=1.0):
+    s = (0.2 + 0.3 * torch.rand(shape, generator=g, device="cuda")) * scale
+    return _pairs(s, -7.5 * s * (0.7 + 0.6 * torch.rand(shape, generator=g, device="cuda")))
+
+
+def _given_logits(logits):
+    """Constant key rows of 128 or 64 elements that meet queries of ones, at scale 1 / D, in these logits."""
+    return _pairs(torch.full_like(logits, LEAST), logits)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("group,ql", [(4, 1), (12, 1), (4, 8)])
+@pytest.mark.parametrize("logit,value", [(70.0, 2.0 ** 40), (87.0, 2.0 ** 22), (87.0, -3.0), (300.0, 2.0 ** 15), (9.0, 2.0 ** 88)])
+def test_a_constant_value_far_above_the_logits_before_it(cuda, dtype, group, ql, logit, value):
+    """A value row without a spread weighs next to nothing, however large its p is; its minimum counts with that p."""
+    if dtype == FP and abs(value) > 60000:
+        value = math.copysign(60000.0, value)
+    B, n, d = 500, 288, 128
+    g = _gen(1)
+    codes = [_codes(g, (B, n, 1, d)) for _ in range(2)]
+    logits = torch.rand(B, n, 1, generator=g, device="cuda") * 2 - 1
+    vp = _plain_pairs(g, (B, n, 1))
+    at = 128 + torch.arange(B, device="cuda") % 120  # in the second run of a warp or later
+    rows = torch.arange(B, device="cuda")
+    logits[rows, at] = logit
+    codes[0].zero_()
+    codes[1][rows, at] = 0
+    vp[rows, at, 0] = torch.tensor([LEAST, value], device="cuda").to(BF)
+    q = torch.ones(B * ql, group, d, device="cuda")
+    _check(q, codes, _given_logits(logits), vp, ql, dtype, scale=1 / d)
