@@ -584,7 +584,8 @@ __global__ void __launch_bounds__(kAttnThreads, AttnInt4Shape<D, NT>::kCtasPerSm
               const float2 sv = make_float2(s[x][nt][2 * half], s[x][nt][2 * half + 1]);
               const float2 dv = kRowScale ? fma2_f32(sv, unscale[nt], nref[nt]) : add2_f32(sv, nref[nt]);
               const float2 p = make_float2(ex2(dv.x), ex2(dv.y));
-              float2 w = mul2_f32(p, mul2_f32(wscale[nt], both(vf[x][half].x)));
+              // In this order, as p * wscale is finite and zero where p is: wscale * sv may overflow beside a p of zero.
+              float2 w = mul2_f32(mul2_f32(p, wscale[nt]), both(vf[x][half].x));
               float2 vmh = both(vf[x][half].y);
               if (masked.value) {
                 w.x = sv.x == -INFINITY ? 0.0f : w.x;
@@ -644,9 +645,12 @@ __global__ void __launch_bounds__(kAttnThreads, AttnInt4Shape<D, NT>::kCtasPerSm
             if (!(hw[c] > was + 10.0f || hi[c] > old + kAttnFarLogit)) continue;
             const float now = fmaxf(old, hi[c]);
             const float room = floorf(now - fmaxf(was, hw[c]));
-            const float nws = now == -INFINITY ? 1.0f : __uint_as_float((uint32_t)(fminf(fmaxf(room, -126.0f), 127.0f) + 127.0f) << 23);
+            // At most 2^112: p * wscale stays finite (p is below 2^14 where the references stand), and the least scale,
+            // 2^-126, still gives a weight that fp16 holds with all its bits.
+            const float grow = fminf(fmaxf(room, -126.0f), 112.0f);
+            const float nws = now == -INFINITY ? 1.0f : __uint_as_float((uint32_t)(grow + 127.0f) << 23);
             fl[c] = now == old ? 1.0f : ex2(old - now);
-            fo[c] = fl[c] * (nws / ws[c]);
+            fo[c] = ex2((now == old ? 0.0f : old - now) + (__log2f(nws) - __log2f(ws[c])));  // as one power: its parts leave fp32
             nr[c] = now == -INFINITY ? 0.0f : -now;
             ws[c] = nws;
           }

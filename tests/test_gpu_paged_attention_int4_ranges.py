@@ -163,3 +163,94 @@ def test_a_constant_value_far_above_the_logits_before_it(cuda, dtype, group, ql,
     vp[rows, at, 0] = torch.tensor([LEAST, value], device="cuda").to(BF)
     q = torch.ones(B * ql, group, d, device="cuda")
     _check(q, codes, _given_logits(logits), vp, ql, dtype, scale=1 / d)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("first", ["constant", "zero pair"])
+@pytest.mark.parametrize("wide", [2.0, 8.0, 2000.0])
+@pytest.mark.parametrize("ql", [2, 8])
+def test_a_hidden_wide_row_after_constant_ones(cuda, dtype, first, wide, ql):
+    """Draft j sees the constant rows alone, as the newest token's wide value row is hidden from all but the last."""
+    d, n = 128, ql
+    codes = [torch.zeros(1, n, 2, d, dtype=torch.int64, device="cuda") for _ in range(2)]
+    codes[1][0, -1] = _codes(_gen(2), (2, d))
+    kp = _plain_pairs(_gen(3), (1, n, 2))
+    vp = torch.zeros(1, n, 2, 2, dtype=BF, device="cuda")
+    vp[..., 0], vp[..., 1] = (LEAST, 1.5) if first == "constant" else (0.0, 0.0)
+    vp[0, -1] = torch.tensor([wide, -7.5 * wide], device="cuda").to(BF)
+    q = torch.randn(ql, 8, d, generator=_gen(4), device="cuda")
+    for causal in (True, False):
+        _check(q, codes, kp, vp, ql, dtype, causal=causal)
+    cache, table = _cache(codes, kp, vp, 16, "NHD")
+    out = mas_b200.paged_attention_int4(q.to(dtype), cache, table, torch.tensor([n], dtype=torch.int32, device="cuda"),
+                                        torch.tensor([0, ql], dtype=torch.int32, device="cuda"))
+    assert (out[0] == vp[0, 0, 0, 1]).all()  # one key: its minimum, which the type holds
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("gap", [60.0, 88.0, 200.0])
+def test_a_wide_row_far_below_constant_ones(cuda, dtype, gap):
+    """Wide value rows whose p is next to nothing, or flushed to zero, beside attended constant rows of the same step."""
+    B, n, d = 40, 96, 128
+    g = _gen(5)
+    codes = [_codes(g, (B, n, 2, d)) for _ in range(2)]
+    logits = torch.rand(B, n, 2, generator=g, device="cuda")
+    far = torch.rand(B, n, 2, generator=g, device="cuda") < 0.3
+    logits = torch.where(far, logits - gap, logits)
+    codes[0].zero_()
+    vp = _plain_pairs(g, (B, n, 2), 500.0)
+    vp = torch.where(far[..., None], vp, torch.tensor([LEAST, -2.0], device="cuda").to(BF))
+    codes[1][~far] = 0
+    _check(torch.ones(B, 8, d, device="cuda"), codes, _given_logits(logits), vp, 1, dtype, scale=1 / d)
+
+
+@pytest.mark.parametrize("top", [30.0, 95.0])
+def test_a_constant_row_above_the_widest(cuda, top):
+    """Rows of scales near 2^95 first, then a constant row far above them: the sums are scaled down by less than fp32 holds."""
+    B, n, d = 500, 288, 128
+    g = _gen(6)
+    codes = [_codes(g, (B, n, 1, d)) for _ in range(2)]
+    logits = torch.rand(B, n, 1, generator=g, device="cuda")
+    vp = _plain_pairs(g, (B, n, 1), 2.0 ** 85)
+    at, rows = 128 + torch.arange(B, device="cuda") % 120, torch.arange(B, device="cuda")
+    logits[rows, at] = top
+    codes[0].zero_()
+    codes[1][rows, at] = 0
+    vp[rows, at, 0] = torch.tensor([LEAST, 2.0 ** 80], device="cuda").to(BF)
+    _check(torch.ones(B, 4, d, device="cuda"), codes, _given_logits(logits), vp, 1, BF, scale=1 / d)
+
+
+def _mixed_pairs(g, order, B, n, h, top):
+    """Value rows of scales 2^-30 to 2^top over a cache, a tenth of them constant, a tenth without a pair."""
+    e = torch.linspace(-30, top, n, device="cuda")[None, :, None] + torch.rand(B, n, h, generator=g, device="cuda")
+    if order == "falling":
+        e = e.flip(1)
+    elif order == "shuffled":
+        e = e[:, torch.randperm(n, generator=g, device="cuda")]
+    s = torch.exp2(e)
+    m = -7.5 * s * (0.7 + 0.6 * torch.rand(B, n, h, generator=g, device="cuda"))
+    kind = torch.rand(B, n, h, generator=g, device="cuda")
+    if order == "halves":
+        kind = torch.where(torch.arange(n, device="cuda")[:, None] < n // 2, 0.0, 1.0).expand(B, n, h)
+    constant, none = kind < 0.1, (kind >= 0.1) & (kind < 0.2)
+    s = torch.where(constant, LEAST, s)
+    m = torch.where(constant, torch.randn(B, n, h, generator=g, device="cuda") * torch.exp2(e), m)
+    return torch.where(none[..., None], torch.zeros(2, dtype=BF, device="cuda"), _pairs(s, m)), constant | none
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("order", ["rising", "falling", "shuffled", "halves"])
+@pytest.mark.parametrize("B,n,ql,hq,hkv,d,layout,page_size", [
+    (120, 300, 1, 12, 1, 128, "NHD", 16), (200, 200, 1, 8, 2, 64, "HND", 5), (30, 400, 5, 8, 2, 128, "NHD", 16),
+    (2, 700, 300, 16, 2, 128, "NHD", 24), (2, 450, 300, 16, 2, 64, "HND", 16),
+])
+def test_value_rows_of_unlike_scales(cuda, dtype, order, B, n, ql, hq, hkv, d, layout, page_size):
+    g = _gen(7)
+    codes = [_codes(g, (B, n, hkv, d)) for _ in range(2)]
+    vp, flat = _mixed_pairs(g, order, B, n, hkv, 8)
+    codes[1][flat] = 0
+    kp = _plain_pairs(g, (B, n, hkv))
+    q = torch.randn(B * ql, hq, d, generator=g, device="cuda")
+    for causal in (True, False):
+        _check(q, codes, kp, vp, ql, dtype, causal=causal, layout=layout, page_size=page_size)
+    _check(3 * q, codes, kp, vp, ql, dtype, layout=layout, page_size=page_size)  # a sharp softmax
