@@ -177,9 +177,8 @@ __device__ __forceinline__ void nibbles_fp16(uint32_t w, uint32_t (&p)[4]) {
 }
 
 // One lane's 8 query elements that meet one code word, as the first product's operand: elements that meet odd
-// nibbles are divided by 16. bf16 rows are first scaled by a power of two to a largest element of 2^11 to 2^12, where fp16
-// holds their 8 bits down to 2^-25 of that largest; fp16 rows are taken as they are (an odd element below 2^-10 loses bits
-// past 2^-21).
+// nibbles are divided by 16. The row is first scaled by a power of two to a largest element of 2^11 to 2^12, where fp16
+// holds a bf16 row's 8 bits down to 2^-25 of that largest, and an fp16 row's elements to within 2^-32 of it.
 __device__ __forceinline__ uint4 query_operand(const float (&f)[8], float scale) {
   const float odd = scale * 0.0625f;
   return make_uint4(Elem<__half>::from_f2(f[0] * scale, f[4] * scale), Elem<__half>::from_f2(f[1] * odd, f[5] * odd),
@@ -252,7 +251,6 @@ template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kAttnThreads, AttnInt4Shape<D, NT>::kCtasPerSm)
     attn_int4_kernel(const AttnInt4Args a) {
   using Sh = AttnInt4Shape<D, NT>;
-  constexpr bool kRowScale = std::is_same<T, __nv_bfloat16>::value;
   // fp16 results: the second product's codes are centred (c - 7.5), through one more product with ones that sums the
   // rounded weights; their rounding then meets codes of half the size. bf16 results are rounded 8 times coarser.
   constexpr bool kCentred = std::is_same<T, __half>::value;
@@ -437,8 +435,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnInt4Shape<D, NT>::kCtasPerSm
         most = __uint_as_float(max(__float_as_uint(most), __shfl_xor_sync(0xffffffffu, __float_as_uint(most), z)));
       }
       const uint32_t exponent = min(max(__float_as_uint(most) >> 23, 12u), 254u);
-      const float scale = kRowScale ? __uint_as_float((265u - exponent) << 23) : 1.0f;
-      const float unscale = kRowScale ? __uint_as_float((exponent - 11u) << 23) : 1.0f;
+      const float scale = __uint_as_float((265u - exponent) << 23), unscale = __uint_as_float((exponent - 11u) << 23);
 #pragma unroll
       for (int i = 0; i < D / 32; ++i)
         *reinterpret_cast<uint4*>(smem + hd * Sh::kQHead + ((i * NT + nt) * 32 + lane) * 16) =
@@ -539,7 +536,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnInt4Shape<D, NT>::kCtasPerSm
       const int tb = t0 + kAttnRun * (sub_warp + head_warps * i) + p0 * 16;
       float2 unscale[NT];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) unscale[nt] = kRowScale ? lds_float2(qrow_u + nt * 64 + 8) : both(1.0f);
+      for (int nt = 0; nt < NT; ++nt) unscale[nt] = lds_float2(qrow_u + nt * 64 + 8);
       float2 vf[kPass][2];  // a token's value scale, and its minimum
 #pragma unroll
       for (int x = 0; x < kPass; ++x)
@@ -582,7 +579,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnInt4Shape<D, NT>::kCtasPerSm
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
               const float2 sv = make_float2(s[x][nt][2 * half], s[x][nt][2 * half + 1]);
-              const float2 dv = kRowScale ? fma2_f32(sv, unscale[nt], nref[nt]) : add2_f32(sv, nref[nt]);
+              const float2 dv = fma2_f32(sv, unscale[nt], nref[nt]);
               const float2 p = make_float2(ex2(dv.x), ex2(dv.y));
               // In this order, as p * wscale is finite and zero where p is: wscale * sv may overflow beside a p of zero.
               float2 w = mul2_f32(mul2_f32(p, wscale[nt]), both(vf[x][half].x));

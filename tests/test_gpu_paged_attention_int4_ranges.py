@@ -254,3 +254,15 @@ def test_value_rows_of_unlike_scales(cuda, dtype, order, B, n, ql, hq, hkv, d, l
     for causal in (True, False):
         _check(q, codes, kp, vp, ql, dtype, causal=causal, layout=layout, page_size=page_size)
     _check(3 * q, codes, kp, vp, ql, dtype, layout=layout, page_size=page_size)  # a sharp softmax
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("ql,gain", [(1, 2.0 ** -12), (1, 2.0 ** -18), (5, 2.0 ** -20), (300, 2.0 ** -18)])
+def test_small_fp16_queries_under_a_large_scale(cuda, d, ql, gain):
+    """Queries down among fp16's least numbers keep all their bits in the logits."""
+    B, n, h = 2 if ql > 8 else 60, 310, 2
+    g = _gen(8)
+    codes = [_codes(g, (B, n, h, d)) for _ in range(2)]
+    kp, vp = _plain_pairs(g, (B, n, h)), _plain_pairs(g, (B, n, h))
+    q = torch.randn(B * ql, 16, d, generator=g, device="cuda") * gain
+    _check(q, codes, kp, vp, ql, FP, scale=d ** -0.5 / gain)
