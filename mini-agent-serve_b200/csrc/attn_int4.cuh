@@ -63,7 +63,9 @@ struct AttnInt4Args {
   int64_t qsn, qsh, osn, osh;  // elements
   float* part;                 // [grid][2][heads a CTA][rows a tile * (D + 2)]
   int32_t* desc;               // [grid][kAttnDescInts]; nullptr: no tile can be split
-  float scale_log2;            // softmax scale * log2(e)
+  // softmax scale * log2(e): its sign (0 for 0) enters with the keys' pairs, its size with a query row's scale, so that no
+  // product on the way to a logit is far larger than the larger of the logit and the key
+  float key_sign, row_scale;
   int32_t B, max_blocks, group;
   int32_t page_shift;          // log2(page_size), or -1
   int32_t causal;
@@ -169,6 +171,9 @@ __device__ __forceinline__ float ex2(float x) {
 // A code word's nibbles at bits 0, 4, 8, 12 of each half as fp16 pairs. A nibble c at the foot of a half IS the
 // fp16 denormal c * 2^-24, one nibble up c * 2^-20: two masks a byte, no arithmetic.
 constexpr float kEvenUnit = 16777216.0f, kOddUnit = 1048576.0f;  // 2^24, 2^20: what undoes that
+// A row's sums are kept at 2^-22 of what its scaled queries give, next to a key's size: a key's scale then meets a factor of 4, where
+// one of 2^24 took scales above 2^104 out of fp32.
+constexpr float kSumUnit = 2.38418579e-7f;
 __device__ __forceinline__ void nibbles_fp16(uint32_t w, uint32_t (&p)[4]) {
   p[0] = w & 0x000f000fu;
   p[1] = w & 0x00f000f0u;
@@ -177,12 +182,19 @@ __device__ __forceinline__ void nibbles_fp16(uint32_t w, uint32_t (&p)[4]) {
 }
 
 // One lane's 8 query elements that meet one code word, as the first product's operand: elements that meet odd
-// nibbles are divided by 16. The row is first scaled by a power of two to a largest element of 2^11 to 2^12, where fp16
-// holds a bf16 row's 8 bits down to 2^-25 of that largest, and an fp16 row's elements to within 2^-32 of it.
-__device__ __forceinline__ uint4 query_operand(const float (&f)[8], float scale) {
-  const float odd = scale * 0.0625f;
-  return make_uint4(Elem<__half>::from_f2(f[0] * scale, f[4] * scale), Elem<__half>::from_f2(f[1] * odd, f[5] * odd),
-                    Elem<__half>::from_f2(f[2] * scale, f[6] * scale), Elem<__half>::from_f2(f[3] * odd, f[7] * odd));
+// nibbles are divided by 16. The row has been scaled by a power of two to a largest element of 2^15 to 2^16 (fp16 ends at 65504,
+// which holds 11 bits there), where fp16 holds a bf16 row's 8 bits down to 2^-29 of that largest, and an fp16 row's elements to
+// within 2^-36 of it.
+__device__ __forceinline__ uint4 query_operand(const float (&f)[8]) {
+  constexpr float kOdd = 0.0625f;
+  return make_uint4(Elem<__half>::from_f2(f[0], f[4]), Elem<__half>::from_f2(f[1] * kOdd, f[5] * kOdd),
+                    Elem<__half>::from_f2(f[2], f[6]), Elem<__half>::from_f2(f[3] * kOdd, f[7] * kOdd));
+}
+
+// What takes a row's sums back to logits: 2^exponent times the softmax scale, kept among the normal numbers (a hidden key's
+// -infinity has to survive it; at the upper end, queries above 2^123 under the usual scales, any difference of logits is past any softmax).
+__device__ __forceinline__ float row_unscale(float power, float scale) {
+  return fminf(fmaxf(power * scale, 1.17549435e-38f), 3.40282347e38f);
 }
 
 // The 8x8 matrix of 16-bit elements held as pairs (row lane / 4, columns 2 (lane % 4), + 1), transposed.
@@ -424,26 +436,30 @@ __global__ void __launch_bounds__(kAttnThreads, AttnInt4Shape<D, NT>::kCtasPerSm
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
           f[i][x] = rr < rows_here ? f[i][x] : 0.0f;
-          sum += f[i][x];
           // as bits, so that a NaN is the most
           most = __uint_as_float(max(__float_as_uint(most), __float_as_uint(fabsf(f[i][x]))));
         }
       }
 #pragma unroll
-      for (int z = 1; z < 4; z <<= 1) {
-        sum += __shfl_xor_sync(0xffffffffu, sum, z);
+      for (int z = 1; z < 4; z <<= 1)
         most = __uint_as_float(max(__float_as_uint(most), __shfl_xor_sync(0xffffffffu, __float_as_uint(most), z)));
-      }
-      const uint32_t exponent = min(max(__float_as_uint(most) >> 23, 12u), 254u);
-      const float scale = __uint_as_float((265u - exponent) << 23), unscale = __uint_as_float((exponent - 11u) << 23);
+      const uint32_t exponent = min(max(__float_as_uint(most) >> 23, 16u), 254u);
+      const float scale = __uint_as_float((269u - exponent) << 23);
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i)
-        *reinterpret_cast<uint4*>(smem + hd * Sh::kQHead + ((i * NT + nt) * 32 + lane) * 16) =
-            query_operand(f[i], scale);
+      for (int i = 0; i < D / 32; ++i) {
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          f[i][x] *= scale;
+          sum += f[i][x];
+        }
+        *reinterpret_cast<uint4*>(smem + hd * Sh::kQHead + ((i * NT + nt) * 32 + lane) * 16) = query_operand(f[i]);
+      }
+#pragma unroll
+      for (int z = 1; z < 4; z <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, z);
       if (t == 0) {
         float* dst = qrow + (hd * kRows + nt * 8 + (g & ~1)) * 2 + (g & 1);
-        dst[0] = sum * scale;
-        dst[2] = unscale;
+        dst[0] = sum * kSumUnit;
+        dst[2] = row_unscale(__uint_as_float((exponent - 15u) << 23), a.row_scale * (1.0f / kSumUnit));
       }
     }
     __syncthreads();  // the queries are in shared memory
@@ -467,13 +483,13 @@ __global__ void __launch_bounds__(kAttnThreads, AttnInt4Shape<D, NT>::kCtasPerSm
       if (kCentred) wsum[nt][0] = wsum[nt][1] = wsum[nt][2] = wsum[nt][3] = 0.0f;
     }
 
-    // Run i has landed: each lane turns its token's pairs into what the logits (in units of log2) and the values need.
+    // Run i has landed: each lane turns its token's pairs into what the logits and the values need.
     auto make_factors = [&](int i) {
       const uint32_t stage = ring_u + (i % kAttnStages) * Sh::kStage;
       const uint2 pr = lds64(stage + Sh::kPairs + lane * 8);
       const float sk = __uint_as_float(pr.x << 16), km = __uint_as_float(pr.x & 0xffff0000u);
       const float sv = __uint_as_float(pr.y << 16), vm = __uint_as_float(pr.y & 0xffff0000u);
-      sts128(stage + Sh::kFactors + lane * 16, sk * (a.scale_log2 * kEvenUnit), km * a.scale_log2, sv,
+      sts128(stage + Sh::kFactors + lane * 16, sk * (a.key_sign * (kEvenUnit * kSumUnit)), km * a.key_sign, sv,
              fmaf(kCentre, sv, vm));
       __syncwarp();
     };

@@ -5,7 +5,7 @@
 // brings in, so the products decide, 4 * D flops a row and key, and each key is unpacked once for 256 rows. Here, too, the products
 // run on bare codes (c - 8 in fp16, exact) and the pairs enter in fp32, between them:
 //   y = S' ks + (sum q) kb,  p = 2^(y - M),  l += p,  r += p (mv + 8 sv),  w = fp16(p sv),  O += w (cv - 8),  o = (O + r) / l
-// (ks, kb the key's scale and minimum + 8 scales, times the softmax scale and log2 e). M is one reference for all: the row's
+// (ks, kb the key's scale and minimum + 8 scales; the row's scale holds the softmax scale and log2 e). M is one reference for all: the row's
 // largest log2 of a weight p sv, moved when one passes it by 8.
 //
 // Measured: 911 and 1511 new tokens of 6 K (96/8 heads of 128) take 1292 us against a floor of 393
@@ -66,6 +66,9 @@ struct PromptShape {
 
 enum PromptBar { kKFull = 0, kKEmpty = 2, kVFull = 4, kVEmpty = 6, kSFull = 8, kPFull = 10, kQFull = 12, kOFull = 14, kKeyFac = 16, kValueFac = 20,
                  kDrain = 24, kPromptBars = 26 };
+// The keys' pairs are taken at 2^-16, exact for any bf16 scale, so that a logit's terms, of 128 elements of up to 2^9 each, stay
+// below twice the key's size; the row's scale gives it back.
+constexpr float kPromptSumUnit = 1.52587891e-5f;
 // Up to this spread of the values' scales (log2) in a step, the largest stands for all in the choice of M.
 constexpr float kPromptSpread = 10.0f;
 
@@ -407,12 +410,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
       const int tok = (it.row0 + min(tile * 128 + r, it.rows - 1)) / a.group;
       const int sub = row - tok * a.group;
       const int lim = a.causal ? min(it.rq.n, max(0, it.rq.n - it.rq.qlen + tok + 1)) : it.rq.n;
-      float qsum = 0.0f, unscale = 1.0f;
+      float qsum = 0.0f, unscale = 0.0f;
       if (it.u1 > it.u0) {
-        // The row as fp16, a bf16 one scaled by a power of two to a largest element of 2^11 to 2^12 (as in attn_int4.cuh).
+        // The row as fp16, a bf16 one scaled by a power of two to a largest element of 2^8 to 2^9 (8 bits down to 2^-22 of that
+        // largest, to within 2^-33 of it below): its sums stay next to a key's size (see kPromptSumUnit).
         const uint16_t* src = static_cast<const uint16_t*>(a.q) + (int64_t)(it.rq.q0 + tok) * a.qsn +
                               ((int64_t)it.head * a.group + (here ? sub : 0)) * a.qsh;
-        float scale = 1.0f;
+        float scale = 1.0f, power = 1.0f;
         if (std::is_same<T, __nv_bfloat16>::value) {
           uint32_t most = 0;
 #pragma unroll 4
@@ -423,9 +427,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
             for (int x = 0; x < 8; ++x) most = max(most, __float_as_uint(fabsf(f[x])));
           }
           const uint32_t exponent = min(max(most >> 23, 12u), 254u);
-          scale = __uint_as_float((265u - exponent) << 23);
-          unscale = __uint_as_float((exponent - 11u) << 23);
+          scale = __uint_as_float((262u - exponent) << 23);
+          power = __uint_as_float((exponent - 8u) << 23);
         }
+        unscale = row_unscale(power, a.row_scale * (1.0f / kPromptSumUnit));
 #pragma unroll 4
         for (int c = 0; c < D / 8; ++c) {
           float f[8];
@@ -687,8 +692,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
           __syncwarp();
         } else {
           const float sk = __uint_as_float(pair.x << 16), mk = __uint_as_float(pair.x & 0xffff0000u);
-          x = bad ? CUDART_NAN_F : sk * a.scale_log2;
-          y = bad ? CUDART_NAN_F : fmaf(8.0f, sk, mk) * a.scale_log2;
+          const float unit = a.key_sign * kPromptSumUnit;
+          x = bad ? CUDART_NAN_F : sk * unit;
+          y = bad ? CUDART_NAN_F : fmaf(8.0f, sk, mk) * unit;
         }
         float* fac = reinterpret_cast<float*>(shared + (values ? Sh::kValueFactors : Sh::kKeyFactors) + buf * 1024 + (r >> 1) * 16);
         fac[r & 1] = x;

@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
@@ -1358,7 +1359,9 @@ int mas_paged_attention_int4(const void* query, void* out, float* lse, const Mas
   a.qsh = q_stride_head; a.osn = out_stride_token; a.osh = out_stride_head;
   a.part = static_cast<float*>(workspace);
   a.desc = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + attn_part_bytes(*st, head_size));
-  a.scale_log2 = sm_scale * 1.4426950408889634f;
+  const float scale_log2 = sm_scale * 1.4426950408889634f;
+  a.key_sign = !std::isfinite(scale_log2) ? NAN : scale_log2 > 0.0f ? 1.0f : scale_log2 < 0.0f ? -1.0f : 0.0f;
+  a.row_scale = std::isfinite(scale_log2) && scale_log2 != 0.0f ? std::fabs(scale_log2) : 1.0f;
   a.B = (int32_t)batch_size; a.max_blocks = (int32_t)max_blocks; a.group = (int32_t)(num_q_heads / num_kv_heads);
   a.page_shift = page_shift(a.kv.page_size);
   a.causal = causal ? 1 : 0;

@@ -266,3 +266,29 @@ def test_small_fp16_queries_under_a_large_scale(cuda, d, ql, gain):
     kp, vp = _plain_pairs(g, (B, n, h)), _plain_pairs(g, (B, n, h))
     q = torch.randn(B * ql, 16, d, generator=g, device="cuda") * gain
     _check(q, codes, kp, vp, ql, FP, scale=d ** -0.5 / gain)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("ql", [1, 5, 300])
+@pytest.mark.parametrize("keys,queries,scale", [
+    (2.0 ** 110, 2.0 ** -110, 1.0), (2.0 ** 122, 2.0 ** -122, 1.0), (2.0 ** 124, 2.0 ** -100, 2.0 ** -24),
+    (2.0 ** 124, 2.0 ** -100, -(2.0 ** -24)),
+    (2.0 ** -100, 2.0 ** 110, 2.0 ** -10), (2.0 ** -118, 2.0 ** 117, 1.0), (1.0, 2.0 ** -60, 2.0 ** 60), (1.0, 2.0 ** 60, 2.0 ** -60),
+])
+def test_key_rows_and_queries_at_the_ends_of_their_range(cuda, d, ql, keys, queries, scale):
+    B, n, h = 2 if ql > 8 else 60, 310, 2
+    g = _gen(9)
+    codes = [_codes(g, (B, n, h, d)) for _ in range(2)]
+    kp, vp = _plain_pairs(g, (B, n, h), keys), _plain_pairs(g, (B, n, h))
+    q = torch.randn(B * ql, 16, d, generator=g, device="cuda") * queries
+    _check(q, codes, kp, vp, ql, BF, scale=scale * d ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("ql", [1, 5, 300])
+def test_a_scale_of_zero_weighs_all_keys_alike(cuda, dtype, ql):
+    B, n, h, d = 2 if ql > 8 else 60, 310, 2, 128
+    g = _gen(10)
+    codes = [_codes(g, (B, n, h, d)) for _ in range(2)]
+    kp, vp = _plain_pairs(g, (B, n, h)), _plain_pairs(g, (B, n, h))
+    _check(torch.randn(B * ql, 16, d, generator=g, device="cuda"), codes, kp, vp, ql, dtype, scale=0.0)
