@@ -900,8 +900,9 @@ __global__ void __launch_bounds__(kAttnThreads) attn_int4_join_kernel(const Attn
       for (int i = 0; i < parts; ++i) {
         const float* p = i == 0 ? first : rest + i * 2 * slot;
         const float m = p[kRows * D + 2 * r], l = p[kRows * D + 2 * r + 1];
-        const float f = m == top ? 1.0f : ex2(m - top);
-        sum = fmaf(f, l, sum);
+        // l by the root twice: beside a reference far below (a prompt part of next to no scales) it may be as far above 1.
+        const float root = m == top ? 1.0f : ex2(0.5f * (m - top)), f = root * root;
+        sum = fmaf(l * root, root, sum);
 #pragma unroll
         for (int j = 0; j < kPer; ++j) acc[j] = fmaf(f, p[r * D + j * 32 + lane], acc[j]);
       }

@@ -6,7 +6,9 @@
 // run on bare codes (c - 8 in fp16, exact) and the pairs enter in fp32, between them:
 //   y = S' ks + (sum q) kb,  p = 2^(y - M),  l += p,  r += p (mv + 8 sv),  w = fp16(p sv),  O += w (cv - 8),  o = (O + r) / l
 // (ks, kb the key's scale and minimum + 8 scales; the row's scale holds the softmax scale and log2 e). M is one reference for all: the row's
-// largest log2 of a weight p sv, moved when one passes it by 8.
+// largest log2 of a p g, moved when one passes it by 8. g is what a key may add to a sum: its scale, or its minimum (+ 8 scales) over 2^60,
+// or 2^-96. So weights stay within fp16, r within 2^68 a key whatever the values are (a constant row's scale is 2^-126), l within 2^104,
+// and scales down to 2^-110, or to 2^-74 of their minimum, keep their weights' bits.
 //
 // Measured: 911 and 1511 new tokens of 6 K (96/8 heads of 128) take 1292 us against a floor of 393
 // (products); 1385 with the items dealt to the SMs whole. What bounds it is the softmax warps, two a scheduler, which issue in 36 % of the cycles: of the 1385, their arithmetic is 636 us, exponentials alone 91,
@@ -58,8 +60,8 @@ struct PromptShape {
   static constexpr int kV = 4 * kTile;       // two stages
   static constexpr int kKeyFactors = 6 * kTile;              // [4][64 pairs of keys] {ks, ks, kb, kb}
   static constexpr int kValueFactors = kKeyFactors + 4096;   // [4][64 pairs of keys] {sv, sv, mv + 8 sv, mv + 8 sv}
-  static constexpr int kLogs = kValueFactors + 4096;         // [4][128] log2 sv
-  static constexpr int kSpread = kLogs + 2048;               // [4][4 warps] {largest, smallest log2 sv}
+  static constexpr int kLogs = kValueFactors + 4096;         // [4][128] log2 g
+  static constexpr int kSpread = kLogs + 2048;               // [4][4 warps] {largest, smallest log2 g}
   static constexpr int kBars = kSpread + 128;
   static constexpr int kSmem = kBars + 256 + 1024;  // the operands are aligned to 1024 bytes by hand
 };
@@ -69,7 +71,7 @@ enum PromptBar { kKFull = 0, kKEmpty = 2, kVFull = 4, kVEmpty = 6, kSFull = 8, k
 // The keys' pairs are taken at 2^-16, exact for any bf16 scale, so that a logit's terms, of 128 elements of up to 2^9 each, stay
 // below twice the key's size; the row's scale gives it back.
 constexpr float kPromptSumUnit = 1.52587891e-5f;
-// Up to this spread of the values' scales (log2) in a step, the largest stands for all in the choice of M.
+// Up to this spread of log2 g in a step, the largest stands for all in the choice of M.
 constexpr float kPromptSpread = 10.0f;
 
 // Shared-memory operand descriptor, 128-byte swizzle. K-major: rows of 128 bytes, groups of eight rows `sbo` bytes apart.
@@ -497,8 +499,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
             t1 = fmaxf(t1, fmaxf(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3])));
           }
           const float top = fmaxf(t0, t1) * unscale;
-          // The largest weight's log2: the largest logit and the largest scale where the scales are alike, each weight's
-          // own where they are not (a hidden key's scale must not set the reference of rows that do not see it).
+          // The largest p g's log2: the largest logit and the largest g where the g are alike, each key's own where they are
+          // not (a hidden key's must not set the reference of rows that do not see it).
           float cand = top + lv_max;
           if (!alike) {
             cand = -INFINITY;
@@ -508,9 +510,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
               cand = fmaxf(cand, fmaxf(fmaf(__uint_as_float(s[i]), unscale, lv.x), fmaf(__uint_as_float(s[i + 1]), unscale, lv.y)));
             }
           }
-          // Values of next to no scale (a constant row's is 2^-126) weigh nothing, but their minima do: p stays below 2^68, so
-          // that r holds minima up to 2^40 or so, while scales down to 2^-60 keep their weights' bits.
-          cand = fmaxf(cand, top - 60.0f);
           const bool up = cand > m + 8.0f;
           if (__any_sync(0xffffffffu, up)) {
             const float was = m;
@@ -537,7 +536,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
               }
               tmem_st32(s_addr, w);
             }
-            l *= factor;
+            // M may rise by more than fp32's exponents while l, of up to 2^104 a key, still counts: by its root, twice.
+            const float root = was == m || was == -INFINITY ? 1.0f : ex2(0.5f * (was - m));
+            l = l * root * root;
             r2.x *= factor;
             r2.y *= factor;
           }
@@ -679,7 +680,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
         if (values) {
           x = bad ? 0.0f : sv;
           y = bad ? 0.0f : fmaf(8.0f, sv, mv);
-          const float lv = __log2f(x);
+          const float lv = __log2f(fmaxf(fmaxf(x, fabsf(y) * 8.67361738e-19f), 1.26217745e-29f));  // log2 g: 2^-60, 2^-96
           const bool counts = !bad && j * kPromptKeys + r < it.rq.n;
           *reinterpret_cast<float*>(shared + Sh::kLogs + buf * 512 + r * 4) = lv;
           float hi = counts ? lv : -INFINITY, lo = counts ? lv : INFINITY;

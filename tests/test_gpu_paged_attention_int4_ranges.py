@@ -292,3 +292,48 @@ def test_a_scale_of_zero_weighs_all_keys_alike(cuda, dtype, ql):
     codes = [_codes(g, (B, n, h, d)) for _ in range(2)]
     kp, vp = _plain_pairs(g, (B, n, h)), _plain_pairs(g, (B, n, h))
     _check(torch.randn(B * ql, 16, d, generator=g, device="cuda"), codes, kp, vp, ql, dtype, scale=0.0)
+
+
+@pytest.mark.parametrize("value", [-1e20, 1e26, 1e-30])
+@pytest.mark.parametrize("ql", [1, 8, 1200])
+def test_constant_values_of_any_size(cuda, value, ql):
+    """The same cache through both kernels: the value, off by its rounding and the sums'."""
+    B, n, h, d = 1, 2000, 2, 128
+    g = _gen(11)
+    codes = [_codes(g, (B, n, h, d)) for _ in range(2)]
+    codes[1].zero_()
+    vp = torch.tensor([LEAST, value], device="cuda").to(BF).expand(B, n, h, 2)
+    _check(torch.randn(ql, 16, d, generator=g, device="cuda"), codes, _plain_pairs(g, (B, n, h)), vp, ql, BF)
+
+
+@pytest.mark.parametrize("order", ["all", "mixed"])
+@pytest.mark.parametrize("scale", [2.0 ** -75, 2.0 ** -92, 2.0 ** 90])
+@pytest.mark.parametrize("ql", [1, 300])
+def test_values_of_very_small_and_very_large_scales(cuda, order, scale, ql):
+    B, n, h, d = 2 if ql > 8 else 60, 450, 2, 128
+    g = _gen(12)
+    codes = [_codes(g, (B, n, h, d)) for _ in range(2)]
+    vp = _plain_pairs(g, (B, n, h), scale)
+    if order == "mixed":  # constant rows of the same size between them
+        flat = torch.rand(B, n, h, generator=g, device="cuda") < 0.5
+        vp = torch.where(flat[..., None], torch.tensor([LEAST, 3 * scale], device="cuda").to(BF), vp)
+        codes[1][flat] = 0
+    _check(torch.randn(B * ql, 16, d, generator=g, device="cuda"), codes, _plain_pairs(g, (B, n, h)), vp, ql, BF)
+
+
+@pytest.mark.parametrize("dtype,scale", [(FP, 100.0), (BF, 100.0), (BF, 2.0 ** 40), (BF, 2.0 ** 85)])
+@pytest.mark.parametrize("first", ["zero pairs", "zeros", "wide"])
+@pytest.mark.parametrize("ql", [1, 300])
+def test_wide_values_beside_a_long_stretch_of_nothing(cuda, dtype, scale, first, ql):
+    """Half a context of rows that hold zeros, half of wide ones, cut into parts: the zeros keep their share of the weight."""
+    B, n, h, d = 2, 2500, 2, 128
+    g = _gen(13)
+    codes = [_codes(g, (B, n, h, d)) for _ in range(2)]
+    vp = _plain_pairs(g, (B, n, h), scale)
+    none = torch.arange(n, device="cuda") < n // 2
+    none = (~none if first == "wide" else none)[None, :, None].expand(B, n, h)
+    vp = torch.where(none[..., None], torch.tensor([0.0 if first == "zero pairs" else LEAST, 0.0], device="cuda").to(BF), vp)
+    codes[1][none] = 0
+    q = torch.randn(B * ql, 16, d, generator=g, device="cuda")
+    for causal in (True, False):
+        _check(q, codes, _plain_pairs(g, (B, n, h)), vp, ql, dtype, causal=causal)
