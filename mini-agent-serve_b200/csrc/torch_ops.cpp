@@ -296,7 +296,8 @@ void check_int32(const at::Tensor& t, const char* name, int64_t entries = -1) {
 at::Tensor as_int32(const at::Tensor& t, const char* name) {
   if (t.scalar_type() == at::kInt && t.is_contiguous()) return t;
   TORCH_CHECK_VALUE(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, name, " must be int32 or int64");
-  return t.to(at::kInt).contiguous();
+  // What int32 does not hold becomes its nearest value, which the kernels refuse; a plain cast could name a token or a length.
+  return (t.scalar_type() == at::kLong ? t.clamp(INT32_MIN, INT32_MAX) : t).to(at::kInt).contiguous();
 }
 
 // A dimension of one entry may carry any stride: it is never stepped over.
