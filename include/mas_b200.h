@@ -366,8 +366,10 @@ MAS_API int mas_paged_attention_int4_workspace(int64_t head_size, int64_t* bytes
  * cum_seq_lens_q[b + 1]) (cum_seq_lens_q NULL: query b alone, num_tokens == batch_size) and seq_lens[b]
  * cached tokens, token i on page block_tables[b * table_stride + i / page_size], entry i % page_size. Query j of
  * n_q sees tokens up to seq_lens[b] - n_q + j (causal), or all of them; q head h reads kv head
- * h / (num_q_heads / num_kv_heads). out = softmax(sm_scale * q . k) v, summed in fp32 and rounded once; a query
- * that sees no token gives zeros. lse (nullable), fp32 [num_tokens][num_q_heads]: log2 of the sum of
+ * h / (num_q_heads / num_kv_heads). out = softmax(sm_scale * q . k) v, summed in fp32 (the value codes' weights in
+ * fp16, relative to the row's largest) and rounded once, for values up to 2^90 in size, key rows of any finite size and queries
+ * below 2^123 (larger ones count as that large beside tiny keys). out may be the query memory itself. A query that sees no
+ * token gives zeros. lse (nullable), fp32 [num_tokens][num_q_heads]: log2 of the sum of
  * 2^(log2(e) * sm_scale * q . k), -infinity for a query without tokens. Rows that no request covers are left as
  * they were. Tokens of a page outside [0, num_pages) read as zeros, and lengths that do not fit num_tokens or
  * the table are cut to them; both set MAS_STATUS_KV_SLOT_OUT_OF_RANGE. Takes the place, for a 4-bit cache, of

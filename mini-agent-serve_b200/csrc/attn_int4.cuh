@@ -6,8 +6,9 @@
 // so the matrix products run on the bare codes, exact in 16 bits, and the pairs enter per token in fp32:
 // no key or value is ever rounded. The weights w_t = p_t sv_t are rounded to fp16 for the second product (11 bits
 // where bf16 has 8, whatever the queries' type); their own running reference, apart from the logits', keeps the
-// largest of a row near 1 whatever the scales are. Maxima, sums and products are accumulated in fp32. z is 0
-// for bf16 results and 7.5 for fp16 ones, where the weights' rounding counts: it then meets codes of half the size.
+// largest of a row near 1 down to the least scale, 2^-126 (2^-14 there). p stays below 2^14, so the sums hold values up to
+// 2^90. Maxima, sums and products are accumulated in fp32. z is 0 for bf16 results and 7.5 for fp16 ones, where the weights'
+// rounding counts: it then meets codes of half the size.
 //
 // Work split. The rows of a request that share a kv head (tokens x group, token-major) are cut into tiles of
 // 8 or 16, the tile's keys into units; all units of a launch, requests outermost, form one line that the
@@ -25,8 +26,8 @@
 // staged bytes: the D axis is permuted so that a lane's codes are 16 (8) consecutive bytes of a row. The weights
 // leave the first product's layout for the second's operand by one 8x8 transpose (movmatrix) each.
 //
-// Measured (96/8 heads of 128, graph replays): 256 requests of up to 4 K tokens, a query each, 185 us against a floor of 88
-// (bytes); 48 of up to 8 K with 2 to 8 drafts each (32/8 heads, fp16) 140 (37); what bounds it is issue: 740 warp instructions a run of 32 tokens of a head, 51 % of the
+// Measured (96/8 heads of 128, graph replays): 256 requests of up to 4 K tokens, a query each, 186 us against a floor of 88
+// (bytes); 48 of up to 8 K with 2 to 8 drafts each (32/8 heads, fp16) 141 (37); what bounds it is issue: 740 warp instructions a run of 32 tokens of a head, 51 % of the
 // slots with 12 warps an SM, ALU 42 %, tensor pipe 35 %, DRAM 37 %. 12 heads of 64 with one row each: 27 us (6), latency.
 #pragma once
 

@@ -10,7 +10,7 @@
 // or 2^-96. So weights stay within fp16, r within 2^68 a key whatever the values are (a constant row's scale is 2^-126), l within 2^104,
 // and scales down to 2^-110, or to 2^-74 of their minimum, keep their weights' bits.
 //
-// Measured: 911 and 1511 new tokens of 6 K (96/8 heads of 128) take 1292 us against a floor of 393
+// Measured: 911 and 1511 new tokens of 6 K (96/8 heads of 128) take 1290 us against a floor of 393
 // (products); 1385 with the items dealt to the SMs whole. What bounds it is the softmax warps, two a scheduler, which issue in 36 % of the cycles: of the 1385, their arithmetic is 636 us, exponentials alone 91,
 // factor loads 172. Sixteen softmax warps of half a row a thread took 1798 (104 registers spill), two S buffers of 64 keys a
 // tile 15 % more than this. Keys and values rounded to bf16 on the way in, two instructions less a (row, key), took 924, but were
@@ -45,10 +45,18 @@ constexpr int kPromptSoftmaxRegs = 168, kPromptUnpackRegs = 88;
 constexpr int kPromptRows = 256;  // rows of a CTA's item
 constexpr int kPromptKeys = 128;  // keys of a step
 // Requests with more rows a kv head go to this kernel, in calls with enough rows (over all heads) an SM to pay for the launches.
-// 96/8 heads of 128, this kernel against tiles of 16 rows. 16 requests over 4 K tokens: 72 rows a kv head 131 and 116 us, 96 rows 151
-// and 136, 132 rows 170 and 192, 288 rows 275 and 359. Rows an SM: 28 (4 requests of 132 rows, 4 K) 69 and 64 us, 51 (of 240) 80 and
-// 89; over 600 tokens 111 an SM take 70 and 54, over 15 K 12 an SM 84 and 85.
-// (The least is above the break-even: a call with many rows and no such request pays 7 us for nothing.)
+// This kernel / tiles of 16 rows, us, 96/8 heads of 128 (32/8: within 7 %), over contexts of 600, 4 K and 15 K tokens:
+//   requests x rows a kv head    rows an SM        600            4 K             15 K
+//   1 x 504                          27          53 /  27       66 /  59       113 /  153
+//   4 x 132                          29          45 /  27       71 /  62       148 /  170
+//   4 x 240                          52          52 /  35       83 /  91       164 /  271
+//   4 x 504                         109          64 /  53      114 / 169       276 /  551
+//   16 x 132                        114          49 /  59      167 / 189       492 /  624
+//   16 x 240                        208          53 /  85      186 / 303       508 / 1025
+// 64 rows an SM lies between the break-even over 4 K tokens and that over 600. What a rule on rows gives away is at the other lengths: up to
+// 1.65 times below it over 15 K, 1.2 times above it over 600. (The lengths are the device's; the host knows the tables' width, a bound.)
+// Rows a kv head, 16 requests over 4 K tokens: 72 rows 131 / 116 and 96 rows 151 / 136 with the items whole, 100 rows (32/8 heads) 134 / 151 with
+// the shares equal. A call with many rows and no such request pays 6 to 9 us for nothing.
 constexpr int kAttnSplitRows = 96, kPromptRowsPerSm = 64;
 constexpr int kPromptJoinCtas = 16;  // a CTA's item in the joining kernel (64 cost an empty launch 10 us more)
 
@@ -175,7 +183,7 @@ __device__ __forceinline__ void unpack_row(uint32_t base, int row, const uint32_
   }
 }
 
-// What starting on an item costs (its queries, the first loads' latency), in steps (0, 1, 4 instead: 1295, 1295, 1288 us where 2 takes
+// What starting on an item costs (its queries, the first loads' latency), in steps (0, 1, 4 instead: 1295, 1295, 1288 us where 2 took
 // 1292), and the least share: one step past that (132 rows over 600 tokens: 47 us, 53 with 4, 70 with 8).
 constexpr int kPromptLead = 2, kPromptMinShare = 3;
 
@@ -525,7 +533,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_int4_prompt_kernel(con
                 tmem_st32(o_addr + d * 32, o);
               }
             }
-            if (c > 0) {  // the first half's weights are relative to the old reference
+            if (c > 0) {  // the first half's weights are relative to the old reference: rounded to 11 bits a second time
               uint32_t w[32];
               tmem_ld32(w, s_addr);
               const __half2 by = __float2half2_rn(factor);

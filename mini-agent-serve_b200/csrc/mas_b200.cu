@@ -751,8 +751,8 @@ int launch_attn_int4(AttnInt4Args a, DeviceState* st, void* stream, int enable_p
 template <typename T, int D>
 int run_attn_int4(AttnInt4Args a, DeviceState* st, void* stream, int enable_pdl) {
   // Rows that share a request's kv head, on average: tiles of 8 rows where they do, of 16 otherwise (drafts of 8 to 32 rows
-  // over 4 K tokens: 164 us with 8, 147 with 16, 193 with tiles of 32, which are not built; 12 rows: 253, 186 and 348; one row:
-  // 27, 33 and 49).
+  // over 4 K tokens, when the heights were compared: 164 us with 8, 147 with 16 (141 now), 193 with tiles of 32, which are not built;
+  // 12 rows: 253, 186 and 348; one row: 27, 33 and 49).
   int64_t rows = ceil_div(a.T, a.B) * a.group;
   a.split_rows = INT32_MAX;
   // The lengths are the device's: where some request may have more than kAttnSplitRows rows, the prompt kernel is launched

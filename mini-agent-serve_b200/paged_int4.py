@@ -367,10 +367,12 @@ def paged_attention_int4(query: torch.Tensor, paged_kv_cache, block_tables: torc
     request covers are not written. Decode steps, drafts to verify and prompt chunks go through one call. All lengths stay on
     the device, so a captured call follows them.
 
-    Keys and values enter the products as exact codes, with their scales applied in fp32; sums and softmax
-    are fp32 and the result is rounded once. `sm_scale` defaults to ``head_dim ** -0.5``. With `return_lse`, returns
+    Keys and values enter the products as exact codes, with their scales applied in fp32; sums and softmax statistics
+    are fp32, the weights of the value codes fp16 (relative to the row's largest), and the result is rounded once. Rows of very unlike
+    scales may stand in one cache: values up to 2^90 in size, key rows of any finite size, queries below 2^123 (larger ones count as
+    that large beside tiny keys). `sm_scale` defaults to ``head_dim ** -0.5``. With `return_lse`, returns
     ``(out, lse)``: fp32 ``(tokens, num_q_heads)``, the log2 of the summed exponentials (-inf for a query without keys), as the merging of
-    partial attentions takes it. A page id out of range reads as zeros and lengths that do not fit the table or
+    partial attentions takes it. `out` may be `query` itself. A page id out of range reads as zeros and lengths that do not fit the table or
     `query` are cut to them; both set STATUS_KV_SLOT_OUT_OF_RANGE.
     """
     hnd = _is_hnd(kv_layout)
